@@ -9,6 +9,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "host.h"
 #include "kernels.h"
 #include "piper_mi355x.h"
 
@@ -27,11 +28,9 @@ static_assert(PIPER_QUERY_SCALE_SLOTS == piper::kQueryScaleSlots && PIPER_KEY_SC
 // Static scratch of piper_prepare_static (see device_scratch below).
 static __device__ __align__(256) unsigned char scratch[PIPER_STATIC_SCRATCH_BYTES];
 
-namespace {
+static thread_local char g_last_error[512] = "";
 
-thread_local char g_last_error[512] = "";
-
-int fail(int status, const char* fmt, ...) {
+int piper::fail(int status, const char* fmt, ...) {
   va_list args;
   va_start(args, fmt);
   vsnprintf(g_last_error, sizeof(g_last_error), fmt, args);
@@ -39,9 +38,12 @@ int fail(int status, const char* fmt, ...) {
   return status;
 }
 
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+namespace {
 
-bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
+using piper::aligned16;
+using piper::ceil_div;
+using piper::device_topology;
+using piper::fail;
 
 int check_shape(const piper_shape* s) {
   if (s == nullptr) return fail(PIPER_ERROR_INVALID_ARGUMENT, "shape is NULL");
@@ -102,7 +104,9 @@ int device_scratch(void** address) {
 std::mutex g_topology_mutex;
 int g_topology[kMaxDevices][2] = {};
 
-int device_topology(int* cus, int* xccs) {
+}  // namespace
+
+int piper::device_topology(int* cus, int* xccs) {
   int device = -1;
   hipError_t err = hipGetDevice(&device);
   if (err != hipSuccess) return fail(PIPER_ERROR_HIP, "hipGetDevice failed: %s", hipGetErrorString(err));
@@ -123,6 +127,8 @@ int device_topology(int* cus, int* xccs) {
   *xccs = g_topology[device][1];
   return PIPER_OK;
 }
+
+namespace {
 
 // The key-range split of a call on the current device; without one, every row counted as split, which
 // bounds the workspace on any device.

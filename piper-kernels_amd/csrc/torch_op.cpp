@@ -6,11 +6,6 @@
 // (calls in a row).  Here a call makes two allocations (the output, and one workspace that holds every prepared
 // buffer): the whole public call takes 17 us.  The op's definition, its fake and its autograd stay in Python
 // (torch.library.custom_op), which also runs calls under an explicit launch plan.
-#include <ATen/ATen.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/DeviceGuard.h>
-#include <torch/library.h>
-
 #include <array>
 #include <atomic>
 #include <exception>
@@ -19,9 +14,14 @@
 #include <mutex>
 #include <string>
 
-#include "piper_mi355x.h"
+#include "torch_common.h"
 
 namespace {
+
+using piper_torch::check;
+using piper_torch::dtype_code;
+using piper_torch::native_input;
+using piper_torch::tensor_arg;
 
 enum Operator : int32_t { kPiper = 0, kSage = 1 };
 
@@ -54,30 +54,6 @@ int32_t plan_for(Operator op, const piper_shape& s, bool causal) {
   if (g_plans.size() >= kMaxPlans) g_plans.clear();
   g_plans.emplace(key, plan);
   return plan;
-}
-
-void check(int status, const char* what) {
-  TORCH_CHECK(status == PIPER_OK, what, " failed (status ", status, "): ", piper_last_error());
-}
-
-int32_t dtype_code(const at::Tensor& t) {
-  TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16,
-              "piper_kernels: tensors must use float16 or bfloat16, got ", t.scalar_type());
-  return t.scalar_type() == at::kBFloat16 ? PIPER_BFLOAT16 : PIPER_FLOAT16;
-}
-
-// Any [B, H, S, D] view whose rows are 16-byte aligned is read in place (the strides of axes of size 1 do
-// not count); anything else is copied.  A copy, not contiguous(): that keeps a contiguous view as it is, also
-// one that starts between two 16-byte boundaries.
-at::Tensor native_input(const at::Tensor& t) {
-  bool in_place = (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) == 0 && t.stride(3) == 1;
-  for (int64_t axis = 0; axis < 3; ++axis) in_place = in_place && (t.size(axis) == 1 || t.stride(axis) % 8 == 0);
-  return in_place ? t : t.clone(at::MemoryFormat::Contiguous);
-}
-
-piper_tensor tensor_arg(const at::Tensor& t) {
-  const auto stride = [&](int64_t axis) { return t.size(axis) == 1 ? 0 : t.stride(axis); };
-  return piper_tensor{t.const_data_ptr(), stride(0), stride(1), stride(2)};
 }
 
 // One allocation handed out in 256-byte steps.
@@ -268,6 +244,7 @@ extern "C" __attribute__((visibility("default"))) const char* piper_torch_set_pl
                                                       __FILE__, __LINE__);
       library->impl("piper_attention", &piper_attention);
       library->impl("sage_attention_2pp", &sage_attention_2pp);
+      piper_torch::register_cache_kernels(*library);
       kernels = library.release();
     }
   } catch (const std::exception& e) {

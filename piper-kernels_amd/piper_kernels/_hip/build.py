@@ -1,6 +1,6 @@
 """Compile the gfx950 libraries from ``piper-kernels_amd/csrc`` with hipcc.
 
-``libpiper_mi355x.so`` is the operator's C ABI (``include/piper_mi355x.h``); ``libpiper_probe.so``
+``libpiper_mi355x.so`` is the operators' C ABI (``include/piper_mi355x.h``, ``include/piper_cache.h``); ``libpiper_probe.so``
 holds the measurement probes (``include/piper_probe.h``), which only bench.py and the tests load.
 Both are plain C-ABI shared objects (no torch headers).  ``libpiper_torch.so`` registers the custom
 ops' GPU kernels with torch over that C ABI (host code only).  All are built in-tree next to this file
@@ -22,10 +22,10 @@ INCLUDE = PACKAGE_ROOT.parent / "include"
 BUILD_DIR = PACKAGE_ROOT / "_build"
 LIBRARY_PATH = Path(__file__).resolve().parent / "libpiper_mi355x.so"
 PROBE_LIBRARY_PATH = Path(__file__).resolve().parent / "libpiper_probe.so"
-SOURCES = ("abi.hip", "prep.hip", "attention.hip", "sage2pp.hip")
+SOURCES = ("abi.hip", "prep.hip", "attention.hip", "sage2pp.hip", "cache.hip", "cache_attention.hip")
 PROBE_SOURCES = ("probe.hip",)
 TORCH_LIBRARY_PATH = Path(__file__).resolve().parent / "libpiper_torch.so"
-TORCH_SOURCE = "torch_op.cpp"
+TORCH_SOURCES = ("torch_op.cpp", "torch_cache.cpp")
 OFFLOAD_ARCH = "gfx950"
 
 COMPILE_FLAGS = (
@@ -69,7 +69,7 @@ def _link(compiler: str, objects: list[Path], target: Path, verbose: bool) -> No
 
 
 def _build_torch_library(verbose: bool) -> None:
-    """The torch kernels: one host source, compiled and linked against torch and the operator library."""
+    """The torch kernels: host sources, compiled and linked against torch and the operator library."""
     import torch
 
     root = Path(torch.__file__).resolve().parent
@@ -79,7 +79,7 @@ def _build_torch_library(verbose: bool) -> None:
         ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1",
          "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
          f"-I{root / 'include'}", f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
-         f"-I{rocm / 'include'}", "-I/opt/rocm/include", "-o", str(tmp), str(CSRC / TORCH_SOURCE),
+         f"-I{rocm / 'include'}", "-I/opt/rocm/include", "-o", str(tmp), *(str(CSRC / source) for source in TORCH_SOURCES),
          f"-L{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip",
          f"-L{LIBRARY_PATH.parent}", "-lpiper_mi355x", "-Wl,-rpath,$ORIGIN"],
         verbose,

@@ -219,6 +219,107 @@ class PiperSageAttentionArgs(ctypes.Structure):
     ]
 
 
+# ---- the quantised cache (include/piper_cache.h) ----
+CACHE_ABI_VERSION = 1
+CACHE_PAGE = 64
+CACHE_INT8 = 0  # piper_cache.code
+CACHE_FP8 = 1
+CACHE_EXPORTED_SYMBOLS = (
+    "piper_cache_abi_version",
+    "piper_cache_write",
+    "piper_cache_read",
+    "piper_cache_attention",
+    "piper_cache_attention_workspace_bytes",
+    "piper_cache_select",
+    "piper_cache_select_workspace_bytes",
+)
+
+
+class PiperCache(ctypes.Structure):
+    _fields_ = [
+        ("key", _ptr),
+        ("key_scale", _ptr),
+        ("value", _ptr),
+        ("value_scale", _ptr),
+        ("bounds", _ptr),
+        ("bound_scale", _ptr),
+        ("pages", _i64),
+        ("kv_heads", _i64),
+        ("head_dim", _i32),
+        ("code", _i32),
+    ]
+
+
+class PiperCacheRows(ctypes.Structure):
+    _fields_ = [
+        ("page_table", _ptr),
+        ("starts", _ptr),
+        ("counts", _ptr),
+        ("table_stride", _i64),
+        ("table_width", _i64),
+        ("batch", _i64),
+        ("tokens", _i64),
+    ]
+
+
+class PiperCacheWriteArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32),
+        ("dtype", _i32),
+        ("cache", PiperCache),
+        ("rows", PiperCacheRows),
+        ("key", PiperTensor),
+        ("value", PiperTensor),
+    ]
+
+
+class PiperCacheReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32),
+        ("dtype", _i32),
+        ("cache", PiperCache),
+        ("rows", PiperCacheRows),
+        ("key", _ptr),
+        ("value", _ptr),
+    ]
+
+
+class PiperCacheAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32),
+        ("dtype", _i32),
+        ("scale", ctypes.c_float),
+        ("reserved", _i32),
+        ("heads", _i64),
+        ("cache", PiperCache),
+        ("rows", PiperCacheRows),
+        ("query", PiperTensor),
+        ("mask", _ptr),
+        ("mask_stride_batch", _i64),
+        ("mask_stride_row", _i64),
+        ("selected", _ptr),
+        ("budget", _i64),
+        ("output", _ptr),
+        ("workspace", _ptr),
+        ("workspace_bytes", _i64),
+    ]
+
+
+class PiperCacheSelectArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32),
+        ("dtype", _i32),
+        ("heads", _i64),
+        ("cache", PiperCache),
+        ("rows", PiperCacheRows),
+        ("query", PiperTensor),
+        ("budget", _i64),
+        ("output", _ptr),
+        ("workspace", _ptr),
+        ("workspace_bytes", _i64),
+    ]
+
+
 class LibraryUnavailableError(RuntimeError):
     """The gfx950 HIP library is not built or cannot be opened."""
 
@@ -258,10 +359,33 @@ class NativeLibrary:
         lib.piper_sage_attention_forward.restype = ctypes.c_int
         lib.piper_sage_attention_forward_balanced.argtypes = [ctypes.POINTER(PiperSageAttentionArgs), _ptr]
         lib.piper_sage_attention_forward_balanced.restype = ctypes.c_int
+        for name, args in (
+            ("piper_cache_write", PiperCacheWriteArgs),
+            ("piper_cache_read", PiperCacheReadArgs),
+            ("piper_cache_attention", PiperCacheAttentionArgs),
+            ("piper_cache_select", PiperCacheSelectArgs),
+        ):
+            function = getattr(lib, name)
+            function.argtypes = [ctypes.POINTER(args), _ptr]
+            function.restype = ctypes.c_int
+        for name, args in (
+            ("piper_cache_attention_workspace_bytes", PiperCacheAttentionArgs),
+            ("piper_cache_select_workspace_bytes", PiperCacheSelectArgs),
+        ):
+            function = getattr(lib, name)
+            function.argtypes = [ctypes.POINTER(args), ctypes.POINTER(_i64)]
+            function.restype = ctypes.c_int
+        lib.piper_cache_abi_version.argtypes = []
+        lib.piper_cache_abi_version.restype = ctypes.c_int
         version = lib.piper_abi_version()
         if version != ABI_VERSION:
             raise LibraryUnavailableError(
                 f"{self.path} has ABI version {version}, this package expects {ABI_VERSION}"
+            )
+        version = lib.piper_cache_abi_version()
+        if version != CACHE_ABI_VERSION:
+            raise LibraryUnavailableError(
+                f"{self.path} has cache ABI version {version}, this package expects {CACHE_ABI_VERSION}"
             )
 
     def has_symbol(self, name: str) -> bool:
@@ -341,6 +465,16 @@ class NativeLibrary:
                     "piper_sage_attention_forward_balanced")
 
 
+    def cache_call(self, name: str, args: ctypes.Structure, stream: int) -> None:
+        """One of the cache's launching entry points (``write``, ``read``, ``attention``, ``select``)."""
+        self._check(getattr(self._lib, f"piper_cache_{name}")(ctypes.byref(args), _ptr(stream)), f"piper_cache_{name}")
+
+    def cache_workspace_bytes(self, name: str, args: ctypes.Structure) -> int:
+        """Workspace bytes of ``attention`` or ``select`` for these arguments on the current device."""
+        value = _i64(0)
+        what = f"piper_cache_{name}_workspace_bytes"
+        self._check(getattr(self._lib, what)(ctypes.byref(args), ctypes.byref(value)), what)
+        return int(value.value)
 
 
 @ctypes.CFUNCTYPE(_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i32)
