@@ -390,7 +390,8 @@ int check_attention(const piper_cache_attention_args* a) {
 piper::CacheAttention attention_of(const piper_cache_attention_args& a) {
   return piper::CacheAttention{cache_of(a.cache), rows_of(a.cache, a.rows), input_of(a.query), a.mask, a.mask_stride_batch,
                                a.mask_stride_row, a.selected, a.output, a.scale, static_cast<int32_t>(a.rows.batch),
-                               static_cast<int32_t>(a.heads), static_cast<int32_t>(a.selected != nullptr ? a.budget : 0)};
+                               static_cast<int32_t>(a.heads), static_cast<int32_t>(a.selected != nullptr ? a.budget : 0), 1, 1, nullptr,
+                               nullptr};
 }
 
 int check_select(const piper_cache_select_args* a) {
@@ -444,7 +445,9 @@ extern "C" int piper_cache_read(const piper_cache_read_args* a, void* stream) {
 extern "C" int piper_cache_attention_workspace_bytes(const piper_cache_attention_args* a, int64_t* bytes) {
   if (bytes == nullptr) return fail(PIPER_ERROR_INVALID_ARGUMENT, "bytes is NULL");
   if (int st = check_attention(a)) return st;
-  *bytes = 0;
+  int cus = 0, xccs = 0;
+  if (int st = piper::device_topology(&cus, &xccs)) return st;
+  *bytes = piper::cache_attention_parts(attention_of(*a), a->cache.head_dim, cus).bytes;
   return PIPER_OK;
 }
 
@@ -457,7 +460,17 @@ extern "C" int piper_cache_attention(const piper_cache_attention_args* a, void* 
   if (int st = check_output("output", a->output)) return st;
   if (a->mask != nullptr && (a->mask_stride_batch < 0 || a->mask_stride_row < 0))
     return fail(PIPER_ERROR_INVALID_ARGUMENT, "mask strides must not be negative");
-  return launched(piper::launch_cache_attention(attention_of(*a), form_of(a->cache, a->dtype), static_cast<hipStream_t>(stream)),
+  int cus = 0, xccs = 0;
+  if (int st = piper::device_topology(&cus, &xccs)) return st;
+  piper::CacheAttention attention = attention_of(*a);
+  const piper::CacheParts parts = piper::cache_attention_parts(attention, a->cache.head_dim, cus);
+  if (parts.blocks > kMaxBlocks) return fail(PIPER_ERROR_UNSUPPORTED, "cache call too large for this build");
+  if (int st = check_workspace(a->workspace, a->workspace_bytes, parts.bytes)) return st;
+  attention.parts = parts.parts;
+  attention.part_pages = parts.part_pages;
+  attention.partial = static_cast<float*>(a->workspace);
+  attention.partial_stats = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + parts.stats_offset);
+  return launched(piper::launch_cache_attention(attention, parts, form_of(a->cache, a->dtype), static_cast<hipStream_t>(stream)),
                   "cache attention");
 }
 

@@ -34,6 +34,17 @@ struct CacheAttention {
   void* output;
   float scale;
   int32_t batch, heads, budget;
+  // parts of a unit's pages: at most `parts`, of at least part_pages pages each; their sums [parts, rows, D] and
+  // maxima and totals [parts, rows] in the workspace
+  int32_t parts, part_pages;
+  float* partial;
+  float2* partial_stats;
+};
+
+struct CacheParts {
+  int32_t parts, part_pages;
+  int64_t blocks;               // workgroups
+  int64_t bytes, stats_offset;  // of the workspace
 };
 
 struct CacheSelect {
@@ -55,7 +66,8 @@ int64_t cache_select_scores(const CacheSelect& a);
 
 hipError_t launch_cache_write(const CacheMove& a, CacheForm form, hipStream_t stream);
 hipError_t launch_cache_read(const CacheMove& a, CacheForm form, hipStream_t stream);
-hipError_t launch_cache_attention(const CacheAttention& a, CacheForm form, hipStream_t stream);
+CacheParts cache_attention_parts(const CacheAttention& a, int head_dim, int cus);
+hipError_t launch_cache_attention(const CacheAttention& a, const CacheParts& parts, CacheForm form, hipStream_t stream);
 hipError_t launch_cache_select(const CacheSelect& a, CacheForm form, hipStream_t stream);
 
 #ifdef __HIPCC__

@@ -110,7 +110,10 @@ class Model:
     def attention(self, q, table, starts, counts=None, mask=None, selected=None, scale=None):
         """FP64 output and, per value, how far a kernel's may be from it: half a step of the output type; P rounded
         to a 16-bit float of 11 bits (2^-11 of the sum of p |v|); score errors of FP32 sums of D products, which change
-        each p by twice their size relatively; an FP32 exp2 and the sums (2^-18 of the sum of p |v|)."""
+        each p by twice their size relatively; an FP32 exp2 and the sums (2^-18 of the sum of p |v|).  Where a key's weight
+        is below 2^-29 of the largest, its 16-bit P is a subnormal: with w = p s 2^15 / r, s the key's value scale and r < 2 s'
+        for the largest value scale s' of the pages, w is off by at most 2^-25, the key's part w c r / 2^15 (|c| <= L) by
+        2^-25 r L / 2^15 < 2^-39 s' L: 2^-39 of the largest value a page of the K/V head holds, for each key seen."""
         batch, heads, tokens, d = q.shape
         _, h, _ = self.shape
         scale = d**-0.5 if scale is None else scale
@@ -124,6 +127,7 @@ class Model:
                 continue
             k, v, there = (x.double() if x.dtype is not torch.bool else x for x in self.tokens(table, b, range(n)))
             at = torch.arange(n)
+            largest = v.nan_to_num(nan=0.0).abs().amax((1, 2))  # per K/V head, seen by the row or not
             for i in range(count):
                 if mask is None:
                     sees = at <= start + i
@@ -150,7 +154,7 @@ class Model:
                     out[b, head, i] = (p @ v[kv][use]) / total
                     size = float((k[kv][use].abs() @ qs.abs()).max()) * scale
                     e = 2 * size * (d + 4) * 2.0**-24
-                    spread[b, head, i] = (2.0**-11 + 2.0**-18 + e) * (p @ v[kv][use].abs()) / total
+                    spread[b, head, i] = (2.0**-11 + 2.0**-18 + e) * (p @ v[kv][use].abs()) / total + float(use.sum()) * 2.0**-39 * largest[kv]
         bound = spread + out.abs() * torch.finfo(q.dtype).eps / 2 + (2.0**-25 if q.dtype is torch.float16 else 0.0)
         return out, bound
 
