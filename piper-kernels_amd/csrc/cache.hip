@@ -390,8 +390,8 @@ int check_attention(const piper_cache_attention_args* a) {
 piper::CacheAttention attention_of(const piper_cache_attention_args& a) {
   return piper::CacheAttention{cache_of(a.cache), rows_of(a.cache, a.rows), input_of(a.query), a.mask, a.mask_stride_batch,
                                a.mask_stride_row, a.selected, a.output, a.scale, static_cast<int32_t>(a.rows.batch),
-                               static_cast<int32_t>(a.heads), static_cast<int32_t>(a.selected != nullptr ? a.budget : 0), 1, 1, nullptr,
-                               nullptr};
+                               static_cast<int32_t>(a.heads), static_cast<int32_t>(a.selected != nullptr ? a.budget : 0),
+                               piper::CacheShares::kWhole, 1, 1, 1, 1, nullptr, nullptr, nullptr};
 }
 
 int check_select(const piper_cache_select_args* a) {
@@ -464,13 +464,17 @@ extern "C" int piper_cache_attention(const piper_cache_attention_args* a, void* 
   if (int st = piper::device_topology(&cus, &xccs)) return st;
   piper::CacheAttention attention = attention_of(*a);
   const piper::CacheParts parts = piper::cache_attention_parts(attention, a->cache.head_dim, cus);
-  if (parts.blocks > kMaxBlocks) return fail(PIPER_ERROR_UNSUPPORTED, "cache call too large for this build");
+  if (parts.workgroups > kMaxBlocks) return fail(PIPER_ERROR_UNSUPPORTED, "cache call too large for this build");
   if (int st = check_workspace(a->workspace, a->workspace_bytes, parts.bytes)) return st;
-  attention.parts = parts.parts;
-  attention.part_pages = parts.part_pages;
+  attention.shares = parts.shares;
+  attention.parts = static_cast<int32_t>(parts.parts);
+  attention.blocks_of_unit = static_cast<int32_t>(parts.blocks_of_unit);
+  attention.least_share = static_cast<int32_t>(parts.least_share);
+  attention.workgroups = parts.workgroups;
   attention.partial = static_cast<float*>(a->workspace);
-  attention.partial_stats = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + parts.stats_offset);
-  return launched(piper::launch_cache_attention(attention, parts, form_of(a->cache, a->dtype), static_cast<hipStream_t>(stream)),
+  attention.partial_stats = reinterpret_cast<float2*>(attention.partial + parts.rows * a->cache.head_dim);
+  attention.pieces = reinterpret_cast<piper::CachePieces*>(attention.partial_stats + parts.rows);
+  return launched(piper::launch_cache_attention(attention, form_of(a->cache, a->dtype), static_cast<hipStream_t>(stream)),
                   "cache attention");
 }
 

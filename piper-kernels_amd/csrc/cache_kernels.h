@@ -24,6 +24,15 @@ struct CacheMove {  // a write's inputs or a read's outputs
   int32_t batch;
 };
 
+// How workgroups share out the pages of blocks of query rows: a workgroup per block; `parts` equal parts of each
+// block (fewer where a part would have less than `least_share` pages); or equal shares of all blocks' pages in a line.
+enum class CacheShares : int32_t { kWhole, kEven, kLine };
+
+struct CachePieces {  // of a block: its first in the workspace, and how many; 1: the output is written
+  int64_t first, parts;
+};
+
+// Pieces' sums [piece, row, D], maxima and totals [piece, row] and the blocks' pieces are in the workspace.
 struct CacheAttention {
   Cache cache;
   CacheRows rows;
@@ -34,17 +43,18 @@ struct CacheAttention {
   void* output;
   float scale;
   int32_t batch, heads, budget;
-  // parts of a unit's pages: at most `parts`, of at least part_pages pages each; their sums [parts, rows, D] and
-  // maxima and totals [parts, rows] in the workspace
-  int32_t parts, part_pages;
+  CacheShares shares;
+  int32_t parts, least_share, blocks_of_unit;
+  int64_t workgroups;
   float* partial;
   float2* partial_stats;
+  CachePieces* pieces;  // of each block
 };
 
 struct CacheParts {
-  int32_t parts, part_pages;
-  int64_t blocks;               // workgroups
-  int64_t bytes, stats_offset;  // of the workspace
+  CacheShares shares;
+  int64_t parts, least_share, blocks_of_unit, workgroups;
+  int64_t rows, bytes;  // of the workspace
 };
 
 struct CacheSelect {
@@ -67,7 +77,7 @@ int64_t cache_select_scores(const CacheSelect& a);
 hipError_t launch_cache_write(const CacheMove& a, CacheForm form, hipStream_t stream);
 hipError_t launch_cache_read(const CacheMove& a, CacheForm form, hipStream_t stream);
 CacheParts cache_attention_parts(const CacheAttention& a, int head_dim, int cus);
-hipError_t launch_cache_attention(const CacheAttention& a, const CacheParts& parts, CacheForm form, hipStream_t stream);
+hipError_t launch_cache_attention(const CacheAttention& a, CacheForm form, hipStream_t stream);
 hipError_t launch_cache_select(const CacheSelect& a, CacheForm form, hipStream_t stream);
 
 #ifdef __HIPCC__

@@ -1,7 +1,8 @@
 // The cache operators' torch kernels (libpiper_torch.so): piper_kernels::cache_write, cache_read, cache_attention
 // and cache_select on GPU tensors, over the C ABI of include/piper_cache.h.  The ops' definitions and fakes are
-// in Python (attention/quantized_cache/hip.py), as are the public functions' checks; what the kernels rely on is
-// checked here too, since a program can call the ops themselves.
+// in Python (attention/quantized_cache/hip.py).  Everything the kernels rely on is checked here, before anything is
+// launched: the public functions call these at once and look for the words of a refusal only after one (a good call's
+// checks take 10 us in Python, as long as a short call's kernels).
 #include <optional>
 
 #include "piper_cache.h"
@@ -109,8 +110,8 @@ piper_cache_rows rows_arg(const Place& place, const Tensor& table, const Tensor&
 }
 
 void check_rows_tensor(const Place& place, const Tensor& t, const char* name, int64_t head_dim) {
-  TORCH_CHECK(t.dim() == 4 && t.size(3) == head_dim && t.device() == place.device, "piper_kernels: ", name,
-              " must have shape [batch, heads, tokens, ", head_dim, "] on ", place.device, ", got ", t.sizes());
+  TORCH_CHECK(t.dim() == 4 && t.size(3) == head_dim && t.stride(3) == 1 && t.numel() > 0 && t.device() == place.device, "piper_kernels: ", name,
+              " must have shape [batch, heads, tokens, ", head_dim, "] and a contiguous head dimension on ", place.device, ", got ", t.sizes());
 }
 
 Tensor workspace_of(const Tensor& like, int64_t bytes) {

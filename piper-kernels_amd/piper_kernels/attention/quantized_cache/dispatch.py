@@ -29,6 +29,8 @@ _DTYPES = (torch.float16, torch.bfloat16)
 _CODE_DTYPES = (torch.int8, torch.float8_e4m3fn)
 _HEAD_DIMS = (64, 128)
 _ops = torch.ops.piper_kernels
+_write, _read = _ops.cache_write.default, _ops.cache_read.default
+_attention, _select = _ops.cache_attention.default, _ops.cache_select.default
 
 
 class QuantizedCache(NamedTuple):
@@ -135,6 +137,10 @@ def _check_tokens(operator: str, name: str, tensor: torch.Tensor, head_dim: int,
         raise ValueError(f"{operator} does not accept an empty {name}, got {tuple(tensor.shape)}")
     if tensor.device != device:
         raise ValueError(f"{operator} {name} must be on {device} as the cache is, got {tensor.device}")
+    _check_grad(operator, tensor)
+
+
+def _check_grad(operator: str, tensor: torch.Tensor) -> None:
     if tensor.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{operator} is an inference-only operator and does not support autograd")
 
@@ -145,12 +151,7 @@ def _check_query(operator: str, query: torch.Tensor, kv_heads: int, head_dim: in
         raise ValueError(f"{operator} query heads must be a multiple of the cache's {kv_heads}, got {query.shape[1]}")
 
 
-_ready: set[torch.device] = set()  # devices whose architecture has been looked up
-
-
 def _require_device(operator: str, device: torch.device) -> None:
-    if device in _ready:
-        return
     target = AcceleratorTarget.from_device(device)
     if not target.supports_piper_mi355x:
         raise NotImplementedError(
@@ -161,6 +162,22 @@ def _require_device(operator: str, device: torch.device) -> None:
         load_library()  # raises LibraryUnavailableError (a RuntimeError) if the library is missing
         load_torch_kernels()
         _ready.add(device)
+
+
+_ready: set[torch.device] = set()  # gfx950 devices, once the kernels are loaded
+
+
+def _call(op, args: tuple, device: torch.device, check):
+    """``op(*args)``.  ``check()`` raises what is wrong with a call.  The op's GPU kernel checks everything before it
+    launches anything, so where that is known to run, the words are looked for only after a refusal."""
+    if torch.compiler.is_compiling() or device not in _ready:
+        check()
+        return op(*args)
+    try:
+        return op(*args)
+    except Exception:
+        check()
+        raise
 
 
 def cache_write(
@@ -181,18 +198,23 @@ def cache_write(
     and of nothing else.
     """
     operator = "cache_write"
-    _, h, d, device = _check_cache(operator, cache)
-    _check_tokens(operator, "key", key, d, device)
-    _check_tokens(operator, "value", value, d, device)
-    if key.shape != value.shape or key.dtype is not value.dtype:
-        raise ValueError(
-            f"{operator} key and value must share shape and dtype, got {key.dtype} {tuple(key.shape)} and {value.dtype} {tuple(value.shape)}"
-        )
-    if key.shape[1] != h:
-        raise ValueError(f"{operator} key and value must have the cache's {h} heads, got {key.shape[1]}")
-    _check_rows(operator, page_table, starts, counts, key.shape[0], device)
-    _require_device(operator, device)
-    _ops.cache_write(key, value, *cache, page_table, starts, counts)
+
+    def check() -> None:
+        _, h, d, device = _check_cache(operator, cache)
+        _check_tokens(operator, "key", key, d, device)
+        _check_tokens(operator, "value", value, d, device)
+        if key.shape != value.shape or key.dtype is not value.dtype:
+            raise ValueError(
+                f"{operator} key and value must share shape and dtype, got {key.dtype} {tuple(key.shape)} and {value.dtype} {tuple(value.shape)}"
+            )
+        if key.shape[1] != h:
+            raise ValueError(f"{operator} key and value must have the cache's {h} heads, got {key.shape[1]}")
+        _check_rows(operator, page_table, starts, counts, key.shape[0], device)
+        _require_device(operator, device)
+
+    _check_grad(operator, key)
+    _check_grad(operator, value)
+    _call(_write, (key, value, *cache, page_table, starts, counts), key.device, check)
 
 
 def cache_read(
@@ -207,16 +229,19 @@ def cache_read(
     """Keys and values of positions ``starts[b] + i`` as ``[batch, kv_heads, size, head_dim]`` in ``dtype`` (FP16 or BF16):
     the values that the codes stand for, rounded once; zero where ``i >= counts[b]`` or the table names no page."""
     operator = "cache_read"
-    _, _, _, device = _check_cache(operator, cache)
-    if dtype not in _DTYPES:
-        raise ValueError(f"{operator} dtype must be float16 or bfloat16, got {dtype}")
-    if size <= 0:
-        raise ValueError(f"{operator} size must be positive, got {size}")
-    if page_table.ndim != 2 or page_table.shape[0] == 0:
-        raise ValueError(f"{operator} page_table must be an int32 tensor of shape [batch, pages], got {tuple(page_table.shape)}")
-    _check_rows(operator, page_table, starts, counts, page_table.shape[0], device)
-    _require_device(operator, device)
-    return _ops.cache_read(*cache[:4], page_table, starts, counts, size, dtype)
+
+    def check() -> None:
+        _, _, _, device = _check_cache(operator, cache)
+        if dtype not in _DTYPES:
+            raise ValueError(f"{operator} dtype must be float16 or bfloat16, got {dtype}")
+        if size <= 0:
+            raise ValueError(f"{operator} size must be positive, got {size}")
+        if page_table.ndim != 2 or page_table.shape[0] == 0:
+            raise ValueError(f"{operator} page_table must be an int32 tensor of shape [batch, pages], got {tuple(page_table.shape)}")
+        _check_rows(operator, page_table, starts, counts, page_table.shape[0], device)
+        _require_device(operator, device)
+
+    return _call(_read, (*cache[:4], page_table, starts, counts, size, dtype), page_table.device, check)
 
 
 def cache_attention(
@@ -246,32 +271,36 @@ def cache_attention(
     Scores, softmax statistics and sums are FP32.  Rows that see nothing are zero.  Inference only.
     """
     operator = "cache_attention"
-    _, h, d, device = _check_cache(operator, cache)
-    _check_query(operator, query, h, d, device)
-    batch, _, tokens, _ = query.shape
-    _check_rows(operator, page_table, starts, counts, batch, device)
-    if mask is not None:
+
+    def check() -> None:
+        _, h, d, device = _check_cache(operator, cache)
+        _check_query(operator, query, h, d, device)
+        batch, _, tokens, _ = query.shape
+        _check_rows(operator, page_table, starts, counts, batch, device)
+        if mask is not None:
+            if selected is not None:
+                raise ValueError(f"{operator} takes a mask or selected pages, not both")
+            if mask.dtype is not torch.bool or mask.ndim != 3 or mask.shape[0] not in (1, batch) or mask.shape[1:] != (tokens, tokens):
+                raise ValueError(
+                    f"{operator} mask must be a bool tensor of shape [{batch} or 1, {tokens}, {tokens}], got {mask.dtype} {tuple(mask.shape)}"
+                )
+            if mask.device != device:
+                raise ValueError(f"{operator} mask must be on {device} as the cache is, got {mask.device}")
         if selected is not None:
-            raise ValueError(f"{operator} takes a mask or selected pages, not both")
-        if mask.dtype is not torch.bool or mask.ndim != 3 or mask.shape[0] not in (1, batch) or mask.shape[1:] != (tokens, tokens):
-            raise ValueError(
-                f"{operator} mask must be a bool tensor of shape [{batch} or 1, {tokens}, {tokens}], got {mask.dtype} {tuple(mask.shape)}"
-            )
-        if mask.device != device:
-            raise ValueError(f"{operator} mask must be on {device} as the cache is, got {mask.device}")
-    if selected is not None:
-        if selected.dtype is not torch.int32 or selected.ndim != 4 or selected.shape[:3] != (batch, h, tokens) or selected.shape[3] == 0:
-            raise ValueError(
-                f"{operator} selected must be an int32 tensor of shape [{batch}, {h}, {tokens}, budget], "
-                f"got {selected.dtype} {tuple(selected.shape)}"
-            )
-        if selected.device != device:
-            raise ValueError(f"{operator} selected must be on {device} as the cache is, got {selected.device}")
-    converted = d**-0.5 if scale is None else float(scale)
-    if not math.isfinite(converted) or converted <= 0:
-        raise ValueError(f"{operator} scale must be finite and positive, got {scale}")
-    _require_device(operator, device)
-    return _ops.cache_attention(query, *cache[:4], page_table, starts, counts, mask, selected, converted)
+            if selected.dtype is not torch.int32 or selected.ndim != 4 or selected.shape[:3] != (batch, h, tokens) or selected.shape[3] == 0:
+                raise ValueError(
+                    f"{operator} selected must be an int32 tensor of shape [{batch}, {h}, {tokens}, budget], "
+                    f"got {selected.dtype} {tuple(selected.shape)}"
+                )
+            if selected.device != device:
+                raise ValueError(f"{operator} selected must be on {device} as the cache is, got {selected.device}")
+        if not math.isfinite(converted) or converted <= 0:
+            raise ValueError(f"{operator} scale must be finite and positive, got {scale}")
+        _require_device(operator, device)
+
+    _check_grad(operator, query)
+    converted = float(scale) if scale is not None else query.shape[3] ** -0.5 if query.ndim == 4 and query.shape[3] else 1.0
+    return _call(_attention, (query, *cache[:4], page_table, starts, counts, mask, selected, converted), query.device, check)
 
 
 def cache_select(
@@ -293,10 +322,14 @@ def cache_select(
     evaluation.
     """
     operator = "cache_select"
-    _, h, d, device = _check_cache(operator, cache)
-    _check_query(operator, query, h, d, device)
-    _check_rows(operator, page_table, starts, counts, query.shape[0], device)
-    if budget <= 0:
-        raise ValueError(f"{operator} budget must be positive, got {budget}")
-    _require_device(operator, device)
-    return _ops.cache_select(query, cache.bounds, cache.bound_scale, page_table, starts, counts, budget)
+
+    def check() -> None:
+        _, h, d, device = _check_cache(operator, cache)
+        _check_query(operator, query, h, d, device)
+        _check_rows(operator, page_table, starts, counts, query.shape[0], device)
+        if budget <= 0:
+            raise ValueError(f"{operator} budget must be positive, got {budget}")
+        _require_device(operator, device)
+
+    _check_grad(operator, query)
+    return _call(_select, (query, cache.bounds, cache.bound_scale, page_table, starts, counts, budget), query.device, check)

@@ -134,6 +134,19 @@ ATTENTION = [
 ]
 
 
+# more pages than one workgroup takes: parts of a sequence's pages, or shares of all sequences', joined afterwards
+LONG = [
+    ((2500,), None, 1, 8, 2, 128, BF16, INT8, "bhtd"),
+    ((2100,), (3,), 5, 8, 2, 64, FP16, FP8, "bthd"),  # 17 to 32 rows a K/V head, two of five tokens padding
+    ((1800,), None, 40, 8, 2, 128, FP16, INT8, "bthd"),  # more than 32
+    ((3000, 5, 0, 1700, -20), (1, 1, 0, 1, 1), 1, 6, 2, 64, BF16, INT8, "bhtd"),  # no row, and rows that see nothing
+    ((1500, 40, 900), (40, 40, 13), 40, 8, 2, 128, BF16, FP8, "bhtd"),
+    (tuple((37 * b * b) % 1300 for b in range(70)), None, 1, 4, 1, 64, FP16, FP8, "bhtd"),  # more sequences than lanes
+    (tuple((211 * b) % 1100 for b in range(67)), tuple(b % 4 for b in range(67)), 3, 4, 1, 64, BF16, INT8, "bhtd"),
+    ((1100, 1300), None, 130, 2, 2, 64, FP16, INT8, "odd"),
+]
+
+
 def _filled(case, seed: int = 11):
     """A cache that holds a case's tokens among bytes that mean nothing (NaN scales, FP8 NaN codes)."""
     starts, counts, rows, _, heads, d, dtype, codes, _ = case
@@ -151,7 +164,11 @@ def _filled(case, seed: int = 11):
     return model, table, ints(*starts), None if counts is None else ints(*counts)
 
 
-@pytest.mark.parametrize("case", ATTENTION, ids=str)
+def _name(case) -> str:
+    return str(case) if len(case[0]) < 10 else f"{len(case[0])} sequences {case[2:]}"
+
+
+@pytest.mark.parametrize("case", ATTENTION + LONG, ids=_name)
 def test_attention(case, gfx950_device) -> None:
     log(f"[case] cache attention {case}")
     model, *where = _filled(case)
@@ -164,7 +181,7 @@ def test_attention(case, gfx950_device) -> None:
         near(got, *model.attention(q, *where, scale=scale))
 
 
-@pytest.mark.parametrize("case", [c for c in ATTENTION if c[2] > 1] + [((63,), None, 1, 2, 1, 64, FP16, INT8, "bhtd")], ids=str)
+@pytest.mark.parametrize("case", [c for c in ATTENTION + LONG if c[2] > 1] + [((63,), None, 1, 2, 1, 64, FP16, INT8, "bhtd")], ids=_name)
 def test_attention_to_a_tree(case, gfx950_device) -> None:
     log(f"[case] cache attention, tree {case}")
     model, *where = _filled(case, 31)
@@ -188,7 +205,7 @@ def _strided(mask, device):
     return wide[:, :, ::2]
 
 
-@pytest.mark.parametrize("case", ATTENTION, ids=str)
+@pytest.mark.parametrize("case", ATTENTION + LONG[:5], ids=_name)
 def test_attention_to_selected_pages(case, gfx950_device) -> None:
     """Lists in any order, with pages named twice, pages after the row's own, beyond the table and negative ones."""
     log(f"[case] cache attention, selected {case}")
@@ -197,7 +214,7 @@ def test_attention_to_selected_pages(case, gfx950_device) -> None:
     b = len(starts)
     q = tokens_of(b, hq, rows, d, dtype, 21, layout)
     cache, dev = cache_of(model, gfx950_device), on(gfx950_device, *where)
-    for budget in (1, 2, 5, 19):
+    for budget in (1, 2, 5, 19, 70):
         g = torch.Generator().manual_seed(budget)
         selected = torch.randint(-1, where[0].shape[1] + 2, (b, heads, rows, budget), generator=g, dtype=torch.int32)
         selected[0, 0, 0] = -1  # nothing at all
