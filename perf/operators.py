@@ -221,10 +221,11 @@ def run(state):
     op, cache = state["op"], state["cache"]
     where = (state["table"], state["starts"], state["counts"])
     if own:
-        package = str(Path(__file__).resolve().parents[1] / "piper-kernels_amd")
-        if package not in sys.path:
-            sys.path.insert(0, package)
-        from piper_kernels import QuantizedCache, cache_attention, cache_read, cache_select, cache_write
+        try:
+            from piper_kernels import QuantizedCache, cache_attention, cache_read, cache_select, cache_write
+        except ImportError:  # the first call
+            sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "piper-kernels_amd"))
+            from piper_kernels import QuantizedCache, cache_attention, cache_read, cache_select, cache_write
 
         cache = QuantizedCache(**cache)
         if op == "write":
