@@ -108,126 +108,315 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheMove a) {
 }
 
 // ---- selection ------------------------------------------------------------------------------------------------------
+//
+// A score's sum over the features of max(c, 0) upper + min(c, 0) lower is one integer product of a page's bounds, which
+// lie in memory as the 2 D bytes that a 16x16x64 instruction takes row by row, with [q+, q-].  Its columns are a K/V
+// head's query heads, token by token; the maximum over a token's columns is one over lanes.  The scores go to LDS and a
+// wave (or for one token all waves) picks the token's pages from registers: the last one's score is found bit by bit,
+// counting with ballots, and the pages come out in their order.  Reading the bounds is what a single token's call has to
+// do; in a chunk the picking, about 20 counts of n / 64 ballots a row, costs as much.
 
-// Scores of a row's earlier pages: one workgroup per row and K/V head, a thread per page.
-template <bool kBf16, int kDim>
-__global__ __launch_bounds__(256) void cache_score_kernel(CacheSelect a) {
-  __shared__ int8_t codes[2 * kDim];  // q+ beside the upper bound, q- beside the lower one
-  __shared__ float scale;
-  const int64_t row = blockIdx.x;
-  const int64_t i = row % a.rows.tokens, unit = row / a.rows.tokens;
-  const int64_t b = unit / a.cache.kv_heads, h = unit % a.cache.kv_heads;
-  const int64_t end = a.rows.end(b, i);
-  const int group = a.heads / a.cache.kv_heads;
-  const int earlier = i < a.rows.count(b) && end > 0 ? static_cast<int>((end - 1) / kPage) : 0;
-  float* const scores = a.scores + row * a.rows.table_width;
-  for (int g = 0; g < group; ++g) {
-    __syncthreads();
-    if (threadIdx.x < kWave) {
-      const uint16_t* q = static_cast<const uint16_t*>(a.query.data) + b * a.query.stride_batch +
-                          (h * group + g) * a.query.stride_head + i * a.query.stride_seq;
-      float x[kDim / kWave], top = 0.0f;
-      bool finite = true;
-      for (int e = 0; e < kDim / kWave; ++e) {
-        x[e] = widen<kBf16>(q[threadIdx.x + e * kWave]);
-        top = fmaxf(top, fabsf(x[e]));
-        finite = finite && is_finite(x[e]);
-      }
-      const RowCode code = row_code<false>(wave_max(top), __all(finite));
-      for (int e = 0; e < kDim / kWave; ++e) {
-        const int8_t c = static_cast<int8_t>(code_of_value<false>(x[e], code.inv));
-        codes[threadIdx.x + e * kWave] = c > 0 ? c : 0;
-        codes[kDim + threadIdx.x + e * kWave] = c < 0 ? c : 0;
-      }
-      if (threadIdx.x == 0) scale = code.scale;
-    }
-    __syncthreads();
-    for (int p = threadIdx.x; p < earlier; p += 256) {
-      const int64_t page = a.rows.page(b, p);
-      const int64_t record = page * a.cache.kv_heads + h;
-      float score = -__builtin_inff();
-      if (page >= 0) {
-        int dot = 0;
-        for (int d = 0; d < 2 * kDim; ++d) dot += static_cast<int>(a.cache.bounds[record * 2 * kDim + d]) * codes[d];
-        score = __fmul_rn(static_cast<float>(dot), scale);
-      }
-      if (g > 0) score = fmaxf(score, scores[p]);
-      if (g == group - 1 && page >= 0) score = __fmul_rn(score, a.cache.bound_scale[record]);
-      scores[p] = score;
-    }
-  }
-}
+typedef int int4_t __attribute__((ext_vector_type(4)));
 
-// Scores in the order of whole numbers: the larger the score, the larger the number (-0 is 0).
+constexpr int kSelectWaves = 8;
+constexpr int kRowScores = 16384;  // scores in LDS: 64 KiB, two workgroups a CU; also what a workgroup's registers hold
+constexpr int kWaveScores = 1024;  // what one wave's registers hold
+
+// Scores in the order of whole numbers: the larger the score, the larger the number (-0 is 0); all of them above 0.
 __device__ __forceinline__ uint32_t score_order(float score) {
   const uint32_t u = __float_as_uint(score + 0.0f);
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// The budget - 1 best earlier pages of a row: the last one's score found eight bits at a time by counting, then the
-// pages above it, and the first of those at it, in their order.
-__global__ __launch_bounds__(256) void cache_select_kernel(CacheSelect a) {
-  __shared__ int counts[256];
-  __shared__ int found[2];
-  __shared__ int wave_above[4], wave_at[4];
-  const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6;
-  const int64_t row = blockIdx.x;
-  const int64_t i = row % a.rows.tokens, unit = row / a.rows.tokens;
-  const int64_t b = unit / a.cache.kv_heads;
+// Where a row of the call stands: its own page, -1 for a row that is none or stands where the table does not reach.
+__device__ __forceinline__ int own_page(const CacheSelect& a, int64_t b, int64_t i) {
+  if (i >= a.rows.count(b)) return -1;
   const int64_t end = a.rows.end(b, i);
-  int32_t* const out = a.output + row * a.budget;
-  // a row that is none, or stands where the table does not reach
-  const bool real = i < a.rows.count(b) && end > 0 && end == a.rows.start(b) + i + 1;
-  const int own = real ? static_cast<int>((end - 1) / kPage) : -1;
-  const int earlier = own > 0 ? own : 0;
-  const int taken = earlier < a.budget - 1 ? earlier : a.budget - 1;
-  const float* const scores = a.scores + row * a.rows.table_width;
-  uint32_t prefix = 0;
-  int left = taken;  // pages still to take among those that share the prefix
-  if (taken < earlier && taken > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      counts[thread] = 0;
-      __syncthreads();
-      for (int p = thread; p < earlier; p += 256) {
-        const uint32_t u = score_order(scores[p]);
-        if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&counts[(u >> shift) & 255u], 1);
+  return end > 0 && end == a.rows.start(b) + i + 1 ? static_cast<int>((end - 1) / kPage) : -1;
+}
+
+// Scores of pages [from, to) for `tokens` rows from `first` on, a wave's tiles of 16 pages being `stride` apart.
+// store(token, page, score).
+template <bool kBf16, int kDim, typename Store>
+__device__ __forceinline__ void score_pages(const CacheSelect& a, int64_t b, int64_t h, int first, int tokens, int columns, int from, int to,
+                                            int stride, Store store) {
+  constexpr int kParts = kDim / 64, kBatch = 4;
+  const int lane = threadIdx.x % kWave, n = lane % 16, g = lane / 16;
+  const int group = a.heads / a.cache.kv_heads;
+  for (int tile = from; tile < to; tile += kBatch * stride) {
+    int4_t bounds[kBatch][2 * kParts];
+    float scale[kBatch];
+    bool there[kBatch];
+#pragma unroll
+    for (int t = 0; t < kBatch; ++t) {
+      const int page = tile + t * stride + n;
+      const int64_t p = page < to ? a.rows.page(b, page) : -1;
+      there[t] = p >= 0;
+      const int64_t record = (there[t] ? p : 0) * a.cache.kv_heads + h;
+      const int8_t* const at = a.cache.bounds + record * 2 * kDim + 16 * g;
+#pragma unroll
+      for (int k = 0; k < 2 * kParts; ++k) bounds[t][k] = *reinterpret_cast<const int4_t*>(at + 64 * k);
+      scale[t] = a.cache.bound_scale[record];
+    }
+    float best[kBatch][4];
+    for (int round = 0; round * columns < group; ++round) {
+      // column n: a head's row in the two halves' codes
+      const int token = first + n / columns, head = round * columns + n % columns;
+      const bool real = n / columns < tokens && head < group;
+      const uint16_t* q = static_cast<const uint16_t*>(a.query.data) + b * a.query.stride_batch;
+      if (real) q += (h * group + head) * a.query.stride_head + token * a.query.stride_seq;
+      float x[kParts][16], top = 0.0f;
+      bool finite = true;
+#pragma unroll
+      for (int k = 0; k < kParts; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float half[8];
+          widen8<kBf16>(*reinterpret_cast<const uint4*>(q + 64 * k + 16 * g + 8 * e), half);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[k][8 * e + i] = half[i];
+            top = fmaxf(top, fabsf(half[i]));
+            finite = finite && is_finite(half[i]);
+          }
+        }
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      const uint64_t good = __ballot(finite);
+      const RowCode code = row_code<false>(top, (good >> n & 0x0001000100010001ull) == 0x0001000100010001ull);
+      int4_t codes[2 * kParts];
+#pragma unroll
+      for (int k = 0; k < kParts; ++k)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t plus = 0, minus = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t c = code_of_value<false>(x[k][4 * w + i], code.inv);
+            plus |= (c < 128 ? c : 0) << (8 * i);
+            minus |= (c < 128 ? 0 : c) << (8 * i);
+          }
+          codes[k][w] = static_cast<int>(plus);
+          codes[kParts + k][w] = static_cast<int>(minus);
+        }
+#pragma unroll
+      for (int t = 0; t < kBatch; ++t) {
+        int4_t dot = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 2 * kParts; ++k) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(bounds[t][k], codes[k], dot, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float s = real ? __fmul_rn(static_cast<float>(dot[i]), code.scale) : -__builtin_inff();
+          best[t][i] = round > 0 ? fmaxf(best[t][i], s) : s;
+        }
       }
-      __syncthreads();
-      if (thread == 0) {
-        int digit = 255, more = left;
-        while (counts[digit] < more) more -= counts[digit--];
-        found[0] = digit;
-        found[1] = more;
+    }
+    // a token's columns, then the pages' scales: row 4 g + i of a tile is its page
+#pragma unroll
+    for (int t = 0; t < kBatch; ++t) {
+      const uint64_t named = __ballot(there[t]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float s = best[t][i];
+        for (int m = columns / 2; m >= 1; m /= 2) s = fmaxf(s, __shfl_xor(s, m, kWave));
+        s = __fmul_rn(s, __shfl(scale[t], 4 * g + i, kWave));
+        const int row = 4 * g + i, page = tile + t * stride + row;
+        if (n % columns == 0 && n / columns < tokens && page < to) store(n / columns, page, named >> row & 1 ? s : -__builtin_inff());
       }
-      __syncthreads();
-      prefix |= static_cast<uint32_t>(found[0]) << shift;
-      left = found[1];
-      __syncthreads();
     }
   }
-  int done = 0, at_done = 0;  // pages taken so far, and how many of them at the last score
-  for (int base = 0; base < earlier && taken > 0; base += 256) {
-    const int p = base + thread;
-    const uint32_t u = p < earlier ? score_order(scores[p]) : 0;
-    const bool all = taken == earlier;
-    const bool above = p < earlier && (all || u > prefix), at = p < earlier && !all && u == prefix;
-    const uint64_t below = (1ull << lane) - 1;
-    const uint64_t at_lanes = __ballot(at);
-    if (lane == 0) wave_at[wave] = __popcll(at_lanes);
-    __syncthreads();
-    int rank = at_done + __popcll(at_lanes & below);
-    for (int w = 0; w < 4; ++w) rank += w < wave ? wave_at[w] : 0, at_done += wave_at[w];
-    const bool take = above || (at && rank < left);
-    const uint64_t lanes = __ballot(take);
-    if (lane == 0) wave_above[wave] = __popcll(lanes);
-    __syncthreads();
-    int place = done + __popcll(lanes & below);
-    for (int w = 0; w < 4; ++w) place += w < wave ? wave_above[w] : 0, done += wave_above[w];
-    if (take) out[place] = p;
-    __syncthreads();
+}
+
+// The count of a workgroup's (kAll) or a wave's lanes' values.
+template <bool kAll>
+__device__ __forceinline__ int count_all(int mine, int* shared, int& turn) {
+  if constexpr (!kAll) return mine;
+  int* const of = shared + (turn++ & 1) * kSelectWaves;  // two in turn: one barrier a count
+  if (threadIdx.x % kWave == 0) of[threadIdx.x / kWave] = mine;
+  __syncthreads();
+  int sum = 0;
+#pragma unroll
+  for (int w = 0; w < kSelectWaves; ++w) sum += of[w];
+  return sum;
+}
+
+// Writes a row's pages: of its `earlier` scores the budget - 1 largest, ties to the lower page, and `own`.  By one wave, or by
+// all of the workgroup's, each with kHeld runs of 64 scores.
+template <bool kAll, int kHeld>
+__device__ __forceinline__ void pick_pages(const float* scores, int own, int budget, int32_t* out, int* shared, int& turn) {
+  const int lane = threadIdx.x % kWave, wave = kAll ? threadIdx.x / kWave : 0;
+  const int earlier = own > 0 ? own : 0, wanted = earlier < budget - 1 ? earlier : budget - 1;
+  const int base = wave * kHeld * kWave;
+  if (wanted == earlier) {  // all of them
+    for (int p = kAll ? threadIdx.x : lane; p < budget; p += kAll ? kWave * kSelectWaves : kWave) out[p] = p <= own ? p : -1;
+    return;
   }
-  if (thread == 0 && real) out[taken] = own;
-  for (int p = taken + (real ? 1 : 0) + thread; p < a.budget; p += 256) out[p] = -1;
+  if (wanted == 0) {  // a budget of one page
+    if ((kAll ? threadIdx.x : lane) == 0) out[0] = own;
+    return;
+  }
+  uint32_t held[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int p = base + k * kWave + lane;
+    held[k] = p < earlier ? score_order(scores[p]) : 0;
+  }
+  // the largest number that at least `wanted` scores reach
+  uint32_t least = 0;
+  int reach = earlier;  // how many do
+  for (int bit = 31; bit >= 0 && reach != wanted; --bit) {
+    const uint32_t next = least | 1u << bit;
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) mine += __popcll(__ballot(held[k] >= next));
+    const int all = count_all<kAll>(mine, shared, turn);
+    if (all >= wanted) {
+      least = next;
+      reach = all;
+    }
+  }
+  // those at it are too many by reach - wanted: the first of them are taken
+  int at = 0, taken = 0, before_at = 0, before = 0;
+  const int spare = reach - wanted;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) at += __popcll(__ballot(held[k] == least));
+  const int all_at = count_all<kAll>(at, shared, turn), left = all_at - spare;
+  if constexpr (kAll) {
+    const int* const of = shared + ((turn - 1) & 1) * kSelectWaves;
+    for (int w = 0; w < wave; ++w) before_at += of[w];
+    const int mine_at = left - before_at < 0 ? 0 : left - before_at < at ? left - before_at : at;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) taken += __popcll(__ballot(held[k] > least));
+    count_all<kAll>(taken + mine_at, shared, turn);
+    const int* const now = shared + ((turn - 1) & 1) * kSelectWaves;
+    for (int w = 0; w < wave; ++w) before += now[w];
+  }
+  const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const uint64_t ties = __ballot(held[k] == least);
+    const bool take = held[k] > least || (held[k] == least && before_at + static_cast<int>(__popcll(ties & below)) < left);
+    before_at += __popcll(ties);
+    const uint64_t lanes = __ballot(take);
+    if (take) out[before + __popcll(lanes & below)] = base + k * kWave + lane;
+    before += __popcll(lanes);
+  }
+  if ((kAll ? threadIdx.x : lane) == 0) out[wanted] = own;
+  for (int p = wanted + 1 + (kAll ? threadIdx.x : lane); p < budget; p += kAll ? kWave * kSelectWaves : kWave) out[p] = -1;
+}
+
+// One workgroup per K/V head and `tokens` rows: scores in LDS, then the rows' pages.
+template <bool kBf16, int kDim>
+__global__ __launch_bounds__(kWave* kSelectWaves) void cache_select_kernel(CacheSelect a, int tokens, int columns) {
+  extern __shared__ float scores[];  // [tokens, table_width]
+  __shared__ int shared[2 * kSelectWaves];
+  const int wave = threadIdx.x / kWave;
+  const int64_t blocks = (a.rows.tokens + tokens - 1) / tokens;
+  const int first = static_cast<int>(blockIdx.x % blocks) * tokens;
+  const int64_t unit = blockIdx.x / blocks, b = unit / a.cache.kv_heads, h = unit % a.cache.kv_heads;
+  const int mine = a.rows.tokens - first < tokens ? a.rows.tokens - first : tokens;
+  int most = 0;
+  for (int t = 0; t < mine; ++t) {
+    const int own = own_page(a, b, first + t);
+    most = own > most ? own : most;
+  }
+  const int width = a.rows.table_width;
+  if (a.budget > 1 && most >= a.budget)  // else every page is taken
+    score_pages<kBf16, kDim>(a, b, h, first, mine, columns, 16 * wave, most, 16 * kSelectWaves,
+                             [&](int token, int page, float score) { scores[token * width + page] = score; });
+  __syncthreads();
+  int turn = 0;
+  int32_t* const out = a.output + (unit * a.rows.tokens + first) * a.budget;
+  if (mine > 1 && most <= kWaveScores) {
+    for (int t = wave; t < mine; t += kSelectWaves) {
+      const int own = own_page(a, b, first + t);
+      if (own <= kWaveScores / 4)
+        pick_pages<false, kWaveScores / 4 / kWave>(scores + t * width, own, a.budget, out + static_cast<int64_t>(t) * a.budget, shared, turn);
+      else
+        pick_pages<false, kWaveScores / kWave>(scores + t * width, own, a.budget, out + static_cast<int64_t>(t) * a.budget, shared, turn);
+    }
+    return;
+  }
+  for (int t = 0; t < mine; ++t) {
+    const int own = own_page(a, b, first + t);
+    if (own <= 4 * kWave * kSelectWaves)
+      pick_pages<true, 4>(scores + t * width, own, a.budget, out + static_cast<int64_t>(t) * a.budget, shared, turn);
+    else
+      pick_pages<true, kRowScores / (kWave * kSelectWaves)>(scores + t * width, own, a.budget, out + static_cast<int64_t>(t) * a.budget, shared, turn);
+  }
+}
+
+// Longer tables, and few rows of long ones: scores in the workspace, by as many workgroups as there are pages for ...
+constexpr int kScoreTiles = 4;  // of 16 pages, a wave
+
+template <bool kBf16, int kDim>
+__global__ __launch_bounds__(256) void cache_score_kernel(CacheSelect a, int columns, int parts) {
+  const int64_t row = blockIdx.x / parts;
+  const int64_t i = row % a.rows.tokens, unit = row / a.rows.tokens;
+  const int64_t b = unit / a.cache.kv_heads, h = unit % a.cache.kv_heads;
+  const int own = own_page(a, b, i);
+  const int from = static_cast<int>(blockIdx.x % parts) * (4 * kScoreTiles * 16) + threadIdx.x / kWave * (kScoreTiles * 16);
+  const int to = own < from + kScoreTiles * 16 ? own : from + kScoreTiles * 16;
+  float* const scores = a.scores + row * a.rows.table_width;
+  if (own >= a.budget)
+    score_pages<kBf16, kDim>(a, b, h, static_cast<int>(i), 1, columns, from, to, 16, [&](int, int page, float score) { scores[page] = score; });
+}
+
+// ... and the row's pages from there: from registers, or where they do not hold them by counting in memory.
+__global__ __launch_bounds__(kWave* kSelectWaves) void cache_pick_kernel(CacheSelect a) {
+  __shared__ int shared[2 * kSelectWaves];
+  const int64_t row = blockIdx.x;
+  const int64_t i = row % a.rows.tokens, b = row / a.rows.tokens / a.cache.kv_heads;
+  const int own = own_page(a, b, i);
+  int32_t* const out = a.output + row * a.budget;
+  const float* const scores = a.scores + row * a.rows.table_width;
+  int turn = 0;
+  if (own <= 4 * kWave * kSelectWaves) {
+    pick_pages<true, 4>(scores, own, a.budget, out, shared, turn);
+    return;
+  }
+  if (own <= kRowScores || a.budget > own) {
+    pick_pages<true, kRowScores / (kWave * kSelectWaves)>(scores, own, a.budget, out, shared, turn);
+    return;
+  }
+  const int wanted = a.budget - 1;
+  uint32_t least = 0;
+  int reach = own;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const auto count = [&](auto holds) {
+    int mine = 0;
+    for (int p = threadIdx.x; p - static_cast<int>(threadIdx.x) < own; p += kWave * kSelectWaves)
+      mine += __popcll(__ballot(p < own && holds(score_order(scores[p < own ? p : 0]))));
+    return count_all<true>(mine, shared, turn);
+  };
+  for (int bit = 31; bit >= 0 && reach != wanted; --bit) {
+    const uint32_t next = least | 1u << bit;
+    const int all = count([&](uint32_t u) { return u >= next; });
+    if (all >= wanted) {
+      least = next;
+      reach = all;
+    }
+  }
+  const int left = count([&](uint32_t u) { return u == least; }) - (reach - wanted);
+  int done = 0, at_done = 0;
+  const uint64_t below = (1ull << lane) - 1;
+  for (int base = 0; base < own; base += kWave * kSelectWaves) {
+    const int p = base + static_cast<int>(threadIdx.x);
+    const uint32_t u = p < own ? score_order(scores[p]) : 0;
+    const uint64_t ties = __ballot(u == least && p < own);
+    const int all_ties = count_all<true>(__popcll(ties), shared, turn);
+    int rank = at_done + __popcll(ties & below);
+    for (int w = 0; w < wave; ++w) rank += shared[((turn - 1) & 1) * kSelectWaves + w];
+    at_done += all_ties;
+    const bool take = p < own && (u > least || (u == least && rank < left));
+    const uint64_t lanes = __ballot(take);
+    const int all_taken = count_all<true>(__popcll(lanes), shared, turn);
+    int place = done + __popcll(lanes & below);
+    for (int w = 0; w < wave; ++w) place += shared[((turn - 1) & 1) * kSelectWaves + w];
+    if (take) out[place] = p;
+    done += all_taken;
+  }
+  if (threadIdx.x == 0) out[wanted] = own;
 }
 
 }  // namespace
@@ -250,19 +439,47 @@ hipError_t launch_cache_read(const CacheMove& a, CacheForm form, hipStream_t str
   });
 }
 
-int64_t cache_select_scores(const CacheSelect& a) {
-  return a.budget > 1 ? static_cast<int64_t>(a.batch) * a.cache.kv_heads * a.rows.tokens * a.rows.table_width : 0;
+// Columns of a token in a score tile: its heads, up to 16, filled up to a power of two.
+static int select_columns(const CacheSelect& a) {
+  const int group = a.heads / a.cache.kv_heads;
+  int columns = 1;
+  while (columns < group && columns < 16) columns *= 2;
+  return columns;
 }
 
-hipError_t launch_cache_select(const CacheSelect& a, CacheForm form, hipStream_t stream) {
-  const dim3 blocks(static_cast<uint32_t>(static_cast<int64_t>(a.batch) * a.cache.kv_heads * a.rows.tokens));
+// Rows of a workgroup whose scores fit its LDS; 0: scores go to the workspace.  That is also the quicker way where there
+// are fewer rows than half the CUs and each has over kSplitPages pages: one workgroup reads a row's bounds at what one CU
+// gets of the memory's rate.
+constexpr int kSplitPages = 1024;
+
+static int select_tokens(const CacheSelect& a, int cus) {
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.cache.kv_heads * a.rows.tokens;
+  if (a.rows.table_width > kRowScores || (2 * rows < cus && a.rows.table_width > kSplitPages)) return 0;
+  return std::min(std::min(16 / select_columns(a), kRowScores / a.rows.table_width), a.rows.tokens);
+}
+
+int64_t cache_select_scores(const CacheSelect& a, int cus) {
+  return select_tokens(a, cus) > 0 ? 0 : static_cast<int64_t>(a.batch) * a.cache.kv_heads * a.rows.tokens * a.rows.table_width;
+}
+
+hipError_t launch_cache_select(const CacheSelect& a, CacheForm form, int cus, hipStream_t stream) {
+  const int64_t units = static_cast<int64_t>(a.batch) * a.cache.kv_heads;
+  const int tokens = select_tokens(a, cus), columns = select_columns(a);
   form.fp8 = false;  // the bounds are INT8 in every cache
   return with_cache_form(form, [&](auto bf16, auto, auto dim) {
-    if (a.budget > 1) {
-      cache_score_kernel<decltype(bf16)::value, decltype(dim)::value><<<blocks, dim3(256), 0, stream>>>(a);
-      if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
+    constexpr bool kBf16 = decltype(bf16)::value;
+    constexpr int kDim = decltype(dim)::value;
+    if (tokens > 0) {
+      const int64_t blocks = units * ceil_div(a.rows.tokens, tokens);
+      cache_select_kernel<kBf16, kDim><<<dim3(static_cast<uint32_t>(blocks)), dim3(kWave * kSelectWaves),
+                                         static_cast<size_t>(tokens) * a.rows.table_width * 4, stream>>>(a, tokens, columns);
+      return hipGetLastError();
     }
-    cache_select_kernel<<<blocks, dim3(256), 0, stream>>>(a);
+    const int parts = static_cast<int>(ceil_div(a.rows.table_width, 4 * kScoreTiles * 16));
+    const int64_t rows = units * a.rows.tokens;
+    cache_score_kernel<kBf16, kDim><<<dim3(static_cast<uint32_t>(rows * parts)), dim3(256), 0, stream>>>(a, columns, parts);
+    if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
+    cache_pick_kernel<<<dim3(static_cast<uint32_t>(rows)), dim3(kWave * kSelectWaves), 0, stream>>>(a);
     return hipGetLastError();
   });
 }
@@ -481,7 +698,9 @@ extern "C" int piper_cache_attention(const piper_cache_attention_args* a, void* 
 extern "C" int piper_cache_select_workspace_bytes(const piper_cache_select_args* a, int64_t* bytes) {
   if (bytes == nullptr) return fail(PIPER_ERROR_INVALID_ARGUMENT, "bytes is NULL");
   if (int st = check_select(a)) return st;
-  *bytes = 4 * piper::cache_select_scores(select_of(*a));
+  int cus = 0, xccs = 0;
+  if (int st = piper::device_topology(&cus, &xccs)) return st;
+  *bytes = 4 * piper::cache_select_scores(select_of(*a), cus);
   return PIPER_OK;
 }
 
@@ -492,6 +711,12 @@ extern "C" int piper_cache_select(const piper_cache_select_args* a, void* stream
   if (int st = check_tensor("query", a->query)) return st;
   if (a->output == nullptr) return fail(PIPER_ERROR_INVALID_ARGUMENT, "output pointer is NULL");
   const piper::CacheSelect select = select_of(*a);
-  if (int st = check_workspace(a->workspace, a->workspace_bytes, 4 * piper::cache_select_scores(select))) return st;
-  return launched(piper::launch_cache_select(select, form_of(a->cache, a->dtype), static_cast<hipStream_t>(stream)), "cache select");
+  int cus = 0, xccs = 0;
+  if (int st = piper::device_topology(&cus, &xccs)) return st;
+  const int64_t scores = piper::cache_select_scores(select, cus);
+  // the score kernel has a workgroup for each 256 pages of a row
+  if (scores / 256 + a->rows.batch * a->heads * a->rows.tokens > kMaxBlocks)
+    return fail(PIPER_ERROR_UNSUPPORTED, "cache call too large for this build");
+  if (int st = check_workspace(a->workspace, a->workspace_bytes, 4 * scores)) return st;
+  return launched(piper::launch_cache_select(select, form_of(a->cache, a->dtype), cus, static_cast<hipStream_t>(stream)), "cache select");
 }

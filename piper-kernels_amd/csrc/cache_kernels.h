@@ -72,13 +72,13 @@ struct CacheForm {
   int head_dim;
 };
 
-int64_t cache_select_scores(const CacheSelect& a);
+int64_t cache_select_scores(const CacheSelect& a, int cus);  // floats of the workspace
 
 hipError_t launch_cache_write(const CacheMove& a, CacheForm form, hipStream_t stream);
 hipError_t launch_cache_read(const CacheMove& a, CacheForm form, hipStream_t stream);
 CacheParts cache_attention_parts(const CacheAttention& a, int head_dim, int cus);
 hipError_t launch_cache_attention(const CacheAttention& a, CacheForm form, hipStream_t stream);
-hipError_t launch_cache_select(const CacheSelect& a, CacheForm form, hipStream_t stream);
+hipError_t launch_cache_select(const CacheSelect& a, CacheForm form, int cus, hipStream_t stream);
 
 #ifdef __HIPCC__
 

@@ -261,7 +261,8 @@ def test_select(case, budget, gfx950_device) -> None:
     same(got, model.select(q, *where, budget), "selected")
 
 
-@pytest.mark.parametrize("width, budget, heads", [(700, 33, 2), (1500, 257, 1), (300, 300, 4), (258, 257, 8)])
+@pytest.mark.parametrize("width, budget, heads", [(700, 33, 2), (1500, 257, 1), (300, 300, 4), (258, 257, 8),
+                                                   (1100, 64, 20), (2300, 5, 7), (16384, 500, 1), (17000, 65, 2), (17000, 16999, 1)])
 def test_select_among_many(width, budget, heads, gfx950_device) -> None:
     """Many pages, ties among them (pages that the table names again, whose scores are equal), entries outside."""
     log(f"[case] cache select among {width}, {budget}")
