@@ -227,23 +227,71 @@ __device__ __forceinline__ void score_pages(const CacheSelect& a, int64_t b, int
   }
 }
 
-// The count of a workgroup's (kAll) or a wave's lanes' values.
+// Counts of all waves (kAll; else of this one).
+constexpr int kCountWords = 2 * kSelectWaves;  // of LDS: two counts in turn, one barrier each
+
 template <bool kAll>
-__device__ __forceinline__ int count_all(int mine, int* shared, int& turn) {
+__device__ __forceinline__ uint4 count_all(uint4 mine, uint4* shared, int& turn) {
   if constexpr (!kAll) return mine;
-  int* const of = shared + (turn++ & 1) * kSelectWaves;  // two in turn: one barrier a count
+  uint4* const of = shared + (turn++ & 1) * kSelectWaves;
   if (threadIdx.x % kWave == 0) of[threadIdx.x / kWave] = mine;
   __syncthreads();
-  int sum = 0;
+  uint4 sum = {0, 0, 0, 0};
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; ++w) sum += of[w];
+  for (int w = 0; w < kSelectWaves; ++w) {
+    const uint4 x = of[w];
+    sum = uint4{sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w};
+  }
   return sum;
+}
+
+template <bool kAll>
+__device__ __forceinline__ int count_all(int mine, uint4* shared, int& turn) {
+  return static_cast<int>(count_all<kAll>(uint4{static_cast<uint32_t>(mine), 0, 0, 0}, shared, turn).x);
+}
+
+// The largest number that at least `wanted` of `all` orders reach, digit by digit from the top, or any that just `wanted`
+// do; `reach`: how many.  count(number) is a wave's count of orders that reach a number.  A digit of kBits costs
+// 2^kBits - 1 counts and, over all waves, one barrier; with kBits > 1
+// two counts share a word, and all stay below 2^16.
+template <bool kAll, int kBits, typename Count>
+__device__ __forceinline__ uint32_t least_order(int wanted, int all, int& reach, uint4* shared, int& turn, Count count) {
+  static_assert(kBits >= 1 && kBits <= 3, "seven counts in four words");
+  uint32_t least = 0;
+  reach = all;
+  for (int shift = 32; shift > 0 && reach != wanted;) {
+    const int bits = shift % kBits == 0 ? kBits : shift % kBits;  // the first digit may be short
+    shift -= bits;
+    uint32_t mine[8] = {};
+#pragma unroll
+    for (int d = 1; d < 1 << kBits; ++d)
+      if (d < 1 << bits) mine[d] = count(least + (static_cast<uint32_t>(d) << shift));
+    if constexpr (kBits == 1) {
+      const int sum = count_all<kAll>(static_cast<int>(mine[1]), shared, turn);
+      if (sum >= wanted) {
+        least += 1u << shift;
+        reach = sum;
+      }
+      continue;
+    }
+    const uint4 sum = count_all<kAll>(uint4{mine[1] | mine[2] << 16, mine[3] | mine[4] << 16, mine[5] | mine[6] << 16, mine[7]}, shared, turn);
+    const uint32_t of[8] = {0, sum.x & 0xffffu, sum.x >> 16, sum.y & 0xffffu, sum.y >> 16, sum.z & 0xffffu, sum.z >> 16, sum.w};
+    int digit = 0;
+#pragma unroll
+    for (int d = 1; d < 1 << kBits; ++d)
+      if (d < 1 << bits && static_cast<int>(of[d]) >= wanted) {
+        digit = d;
+        reach = of[d];
+      }
+    least += static_cast<uint32_t>(digit) << shift;
+  }
+  return least;
 }
 
 // Writes a row's pages: of its `earlier` scores the budget - 1 largest, ties to the lower page, and `own`.  By one wave, or by
 // all of the workgroup's, each with kHeld runs of 64 scores.
 template <bool kAll, int kHeld>
-__device__ __forceinline__ void pick_pages(const float* scores, int own, int budget, int32_t* out, int* shared, int& turn) {
+__device__ __forceinline__ void pick_pages(const float* scores, int own, int budget, int32_t* out, uint4* shared, int& turn) {
   const int lane = threadIdx.x % kWave, wave = kAll ? threadIdx.x / kWave : 0;
   const int earlier = own > 0 ? own : 0, wanted = earlier < budget - 1 ? earlier : budget - 1;
   const int base = wave * kHeld * kWave;
@@ -261,20 +309,13 @@ __device__ __forceinline__ void pick_pages(const float* scores, int own, int bud
     const int p = base + k * kWave + lane;
     held[k] = p < earlier ? score_order(scores[p]) : 0;
   }
-  // the largest number that at least `wanted` scores reach
-  uint32_t least = 0;
-  int reach = earlier;  // how many do
-  for (int bit = 31; bit >= 0 && reach != wanted; --bit) {
-    const uint32_t next = least | 1u << bit;
-    int mine = 0;
+  int reach;
+  const uint32_t least = least_order<kAll, kAll ? kHeld <= 4 ? 3 : 2 : 1>(wanted, earlier, reach, shared, turn, [&](uint32_t number) {
+    uint32_t mine = 0;
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k) mine += __popcll(__ballot(held[k] >= next));
-    const int all = count_all<kAll>(mine, shared, turn);
-    if (all >= wanted) {
-      least = next;
-      reach = all;
-    }
-  }
+    for (int k = 0; k < kHeld; ++k) mine += __popcll(__ballot(held[k] >= number));
+    return mine;
+  });
   // those at it are too many by reach - wanted: the first of them are taken
   int at = 0, taken = 0, before_at = 0, before = 0;
   const int spare = reach - wanted;
@@ -282,14 +323,14 @@ __device__ __forceinline__ void pick_pages(const float* scores, int own, int bud
   for (int k = 0; k < kHeld; ++k) at += __popcll(__ballot(held[k] == least));
   const int all_at = count_all<kAll>(at, shared, turn), left = all_at - spare;
   if constexpr (kAll) {
-    const int* const of = shared + ((turn - 1) & 1) * kSelectWaves;
-    for (int w = 0; w < wave; ++w) before_at += of[w];
+    const uint4* const of = shared + ((turn - 1) & 1) * kSelectWaves;
+    for (int w = 0; w < wave; ++w) before_at += of[w].x;
     const int mine_at = left - before_at < 0 ? 0 : left - before_at < at ? left - before_at : at;
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) taken += __popcll(__ballot(held[k] > least));
     count_all<kAll>(taken + mine_at, shared, turn);
-    const int* const now = shared + ((turn - 1) & 1) * kSelectWaves;
-    for (int w = 0; w < wave; ++w) before += now[w];
+    const uint4* const now = shared + ((turn - 1) & 1) * kSelectWaves;
+    for (int w = 0; w < wave; ++w) before += now[w].x;
   }
   const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
@@ -309,7 +350,7 @@ __device__ __forceinline__ void pick_pages(const float* scores, int own, int bud
 template <bool kBf16, int kDim>
 __global__ __launch_bounds__(kWave* kSelectWaves) void cache_select_kernel(CacheSelect a, int tokens, int columns) {
   extern __shared__ float scores[];  // [tokens, table_width]
-  __shared__ int shared[2 * kSelectWaves];
+  __shared__ uint4 shared[kCountWords];
   const int wave = threadIdx.x / kWave;
   const int64_t blocks = (a.rows.tokens + tokens - 1) / tokens;
   const int first = static_cast<int>(blockIdx.x % blocks) * tokens;
@@ -364,7 +405,7 @@ __global__ __launch_bounds__(256) void cache_score_kernel(CacheSelect a, int col
 
 // ... and the row's pages from there: from registers, or where they do not hold them by counting in memory.
 __global__ __launch_bounds__(kWave* kSelectWaves) void cache_pick_kernel(CacheSelect a) {
-  __shared__ int shared[2 * kSelectWaves];
+  __shared__ uint4 shared[kCountWords];
   const int64_t row = blockIdx.x;
   const int64_t i = row % a.rows.tokens, b = row / a.rows.tokens / a.cache.kv_heads;
   const int own = own_page(a, b, i);
@@ -380,24 +421,20 @@ __global__ __launch_bounds__(kWave* kSelectWaves) void cache_pick_kernel(CacheSe
     return;
   }
   const int wanted = a.budget - 1;
-  uint32_t least = 0;
-  int reach = own;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  // a row of 2^24 pages has counts over 16 bits: one at a time
   const auto count = [&](auto holds) {
     int mine = 0;
-    for (int p = threadIdx.x; p - static_cast<int>(threadIdx.x) < own; p += kWave * kSelectWaves)
+    for (int base = wave * kWave; base < own; base += kWave * kSelectWaves) {
+      const int p = base + lane;
       mine += __popcll(__ballot(p < own && holds(score_order(scores[p < own ? p : 0]))));
-    return count_all<true>(mine, shared, turn);
-  };
-  for (int bit = 31; bit >= 0 && reach != wanted; --bit) {
-    const uint32_t next = least | 1u << bit;
-    const int all = count([&](uint32_t u) { return u >= next; });
-    if (all >= wanted) {
-      least = next;
-      reach = all;
     }
-  }
-  const int left = count([&](uint32_t u) { return u == least; }) - (reach - wanted);
+    return mine;
+  };
+  int reach;
+  const uint32_t least = least_order<true, 1>(wanted, own, reach, shared, turn,
+                                              [&](uint32_t number) { return static_cast<uint32_t>(count([&](uint32_t u) { return u >= number; })); });
+  const int left = count_all<true>(count([&](uint32_t u) { return u == least; }), shared, turn) - (reach - wanted);
   int done = 0, at_done = 0;
   const uint64_t below = (1ull << lane) - 1;
   for (int base = 0; base < own; base += kWave * kSelectWaves) {
@@ -406,13 +443,13 @@ __global__ __launch_bounds__(kWave* kSelectWaves) void cache_pick_kernel(CacheSe
     const uint64_t ties = __ballot(u == least && p < own);
     const int all_ties = count_all<true>(__popcll(ties), shared, turn);
     int rank = at_done + __popcll(ties & below);
-    for (int w = 0; w < wave; ++w) rank += shared[((turn - 1) & 1) * kSelectWaves + w];
+    for (int w = 0; w < wave; ++w) rank += shared[((turn - 1) & 1) * kSelectWaves + w].x;
     at_done += all_ties;
     const bool take = p < own && (u > least || (u == least && rank < left));
     const uint64_t lanes = __ballot(take);
     const int all_taken = count_all<true>(__popcll(lanes), shared, turn);
     int place = done + __popcll(lanes & below);
-    for (int w = 0; w < wave; ++w) place += shared[((turn - 1) & 1) * kSelectWaves + w];
+    for (int w = 0; w < wave; ++w) place += shared[((turn - 1) & 1) * kSelectWaves + w].x;
     if (take) out[place] = p;
     done += all_taken;
   }
@@ -448,13 +485,13 @@ static int select_columns(const CacheSelect& a) {
 }
 
 // Rows of a workgroup whose scores fit its LDS; 0: scores go to the workspace.  That is also the quicker way where there
-// are fewer rows than half the CUs and each has over kSplitPages pages: one workgroup reads a row's bounds at what one CU
+// are no more rows than CUs and each has over kSplitPages pages: one workgroup reads a row's bounds at what one CU
 // gets of the memory's rate.
-constexpr int kSplitPages = 1024;
+constexpr int kSplitPages = 512;
 
 static int select_tokens(const CacheSelect& a, int cus) {
   const int64_t rows = static_cast<int64_t>(a.batch) * a.cache.kv_heads * a.rows.tokens;
-  if (a.rows.table_width > kRowScores || (2 * rows < cus && a.rows.table_width > kSplitPages)) return 0;
+  if (a.rows.table_width > kRowScores || (rows <= cus && a.rows.table_width > kSplitPages)) return 0;
   return std::min(std::min(16 / select_columns(a), kRowScores / a.rows.table_width), a.rows.tokens);
 }
 
