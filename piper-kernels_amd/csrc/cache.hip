@@ -10,13 +10,152 @@
 namespace piper {
 namespace {
 
-// ---- write ----------------------------------------------------------------------------------------------------------
+// ---- write and read -------------------------------------------------------------------------------------------------
+//
+// Both are bound by the bytes they move.  A workgroup has a page of one K/V head, each wave groups of eight of its tokens:
+// lane 8 r + c has an eighth of token r's features, in 32 (D = 128) or 16 consecutive bytes of 16-bit values.  Key
+// codes lie as the lanes have them; value codes change lanes, so that each has all eight tokens of two features or one.
 
-// One wave per page touched and K/V head: token by token, the row's largest magnitude over the lanes, then its codes.
+constexpr int kMoveWaves = 4;
+
+template <int kDim>
+struct Eighth {  // of a token's row
+  static constexpr int kValues = kDim / 8, kLoads = kDim / 64, kWords = kDim / 32;  // 16-byte loads; words of four codes
+};
+
+// Swaps the values of two registers between lanes 32 (16) apart: the lower lanes end with both lanes' `a`, the upper ones
+// with both lanes' `b`, the lower lane's first.
+__device__ __forceinline__ void exchange32(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+
+__device__ __forceinline__ void exchange16(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+
+__device__ __forceinline__ uint32_t lane_xor8(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xf, 0xf, false));  // row_ror:8
+}
+
+// Bytes of two words by selector (0-3: of b, 4-7: of a).
+__device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b, uint32_t selector) { return __builtin_amdgcn_perm(a, b, selector); }
+
+// From lane 8 r + c's codes of token r, features kValues c .. + kValues - 1, those of tokens 0..7 of features
+// (kValues / 8) (8 c + r) .. : halves of the words change lanes with r's top bit, halves of the rest with the next, and the
+// last step, lanes 8 apart, interleaves the even tokens' bytes with the odd ones'.
+template <int kDim>
+__device__ __forceinline__ void tokens_together(const uint32_t (&codes)[kDim / 32], uint32_t (&out)[kDim / 32], int r) {
+  uint32_t mine[kDim / 64], other[kDim / 64];  // tokens t, t + 2 | t + 4, t + 6 (t = r % 2) of this lane's feature(s), and of its partner's
+  if constexpr (kDim == 128) {
+    uint32_t p0 = codes[0], p1 = codes[2], q0 = codes[1], q1 = codes[3];
+    exchange32(p0, p1);
+    exchange32(q0, q1);
+    exchange16(p0, q0);  // tokens t, t + 2
+    exchange16(p1, q1);  // tokens t + 4, t + 6
+    const uint32_t low0 = bytes_of(q0, p0, 0x05040100), high0 = bytes_of(q0, p0, 0x07060302);
+    const uint32_t low1 = bytes_of(q1, p1, 0x05040100), high1 = bytes_of(q1, p1, 0x07060302);
+    mine[0] = r & 1 ? high0 : low0;
+    mine[1] = r & 1 ? high1 : low1;
+    other[0] = lane_xor8(r & 1 ? low0 : high0);
+    other[1] = lane_xor8(r & 1 ? low1 : high1);
+    const uint32_t even0 = r & 1 ? other[0] : mine[0], odd0 = r & 1 ? mine[0] : other[0];
+    const uint32_t even1 = r & 1 ? other[1] : mine[1], odd1 = r & 1 ? mine[1] : other[1];
+    out[0] = bytes_of(odd0, even0, 0x06020400);
+    out[1] = bytes_of(odd1, even1, 0x06020400);
+    out[2] = bytes_of(odd0, even0, 0x07030501);
+    out[3] = bytes_of(odd1, even1, 0x07030501);
+  } else {
+    uint32_t p0 = codes[0], p1 = codes[1];
+    exchange32(p0, p1);  // tokens t, t + 4 (t = r % 4)
+    uint32_t low = bytes_of(p1, p0, 0x05040100), high = bytes_of(p1, p0, 0x07060302);
+    exchange16(low, high);  // tokens t, t + 4 | t + 2, t + 6 (t = r % 2) of two features
+    const uint32_t first = bytes_of(high, low, 0x06020400), second = bytes_of(high, low, 0x07030501);  // tokens t, t + 2, t + 4, t + 6
+    mine[0] = r & 1 ? second : first;
+    other[0] = lane_xor8(r & 1 ? first : second);
+    const uint32_t even = r & 1 ? other[0] : mine[0], odd = r & 1 ? mine[0] : other[0];
+    out[0] = bytes_of(odd, even, 0x05010400);
+    out[1] = bytes_of(odd, even, 0x07030602);
+  }
+}
+
+// Max over the eight lanes of a token.
+__device__ __forceinline__ uint32_t token_max(uint32_t v) {
+  const auto max_with = [&](auto ctrl) {
+    const uint32_t x = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value, 0xf, 0xf, false));
+    v = v > x ? v : x;
+  };
+  max_with(std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
+  max_with(std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
+  max_with(std::integral_constant<int, 0x141>{});  // row_half_mirror
+  return v;
+}
+
+typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
+
+// A token's codes from its 16-bit values, and its scale.  Largest magnitude: the values' bits without the sign are in
+// the order of whole numbers, infinities and NaN above all.
 template <bool kBf16, bool kFp8, int kDim>
-__global__ __launch_bounds__(kWave) void cache_write_kernel(CacheMove a) {
-  constexpr int kPer = kDim / kWave;  // features of a lane
-  const int lane = threadIdx.x;
+__device__ __forceinline__ float encode_row(const uint4 (&raw)[kDim / 64], uint32_t (&codes)[kDim / 32]) {
+  ushort2_t most = {0, 0};
+#pragma unroll
+  for (int k = 0; k < kDim / 64; ++k) {
+    const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(ushort2_t, w[i] & 0x7fff7fffu));
+  }
+  const uint32_t bits = token_max(most.x > most.y ? most.x : most.y);
+  const RowCode code = row_code<kFp8>(widen<kBf16>(static_cast<uint16_t>(bits)), bits < (kBf16 ? 0x7f80u : 0x7c00u));
+#pragma unroll
+  for (int k = 0; k < kDim / 64; ++k) {
+    float x[8];
+    widen8<kBf16>(code.inv == 0.0f ? uint4{0, 0, 0, 0} : raw[k], x);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if constexpr (kFp8) {
+        int packed = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w] * code.inv, x[4 * w + 1] * code.inv, 0, false);
+        codes[2 * k + w] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w + 2] * code.inv, x[4 * w + 3] * code.inv, packed, true));
+      } else {
+        uint32_t c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma clang fp contract(off)  // see code_of_value
+          c[i] = __float_as_uint(x[4 * w + i] * code.inv + kAccBiasValue);
+        }
+        codes[2 * k + w] = bytes_of(bytes_of(c[3], c[2], 0x0c0c0400), bytes_of(c[1], c[0], 0x0c0c0400), 0x05040100);
+      }
+    }
+  }
+  return code.scale;
+}
+
+template <bool kFp8>
+__device__ __forceinline__ void decode4(uint32_t codes, float (&x)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kFp8) {
+      switch (i) {
+        case 0: x[i] = __builtin_amdgcn_cvt_f32_fp8(codes, 0); break;
+        case 1: x[i] = __builtin_amdgcn_cvt_f32_fp8(codes, 1); break;
+        case 2: x[i] = __builtin_amdgcn_cvt_f32_fp8(codes, 2); break;
+        default: x[i] = __builtin_amdgcn_cvt_f32_fp8(codes, 3); break;
+      }
+    } else {
+      x[i] = static_cast<float>(static_cast<int8_t>(codes >> (8 * i)));
+    }
+  }
+}
+
+// Codes of the rows of a page of one K/V head; of a page that they fill also its bounds.
+template <bool kBf16, bool kFp8, int kDim>
+__global__ __launch_bounds__(kWave* kMoveWaves) void cache_write_kernel(CacheMove a) {
+  using E = Eighth<kDim>;
+  __shared__ float ends[kMoveWaves][2][kDim];
+  __shared__ float tops[2];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r = lane / 8, c = lane % 8;
   const int64_t touched = pages_touched(a.rows.tokens);
   const int64_t unit = blockIdx.x / touched;
   const int64_t b = unit / a.cache.kv_heads, h = unit % a.cache.kv_heads;
@@ -25,86 +164,182 @@ __global__ __launch_bounds__(kWave) void cache_write_kernel(CacheMove a) {
   const int64_t page = a.rows.page(b, logical);
   if (in.n == 0 || page < 0) return;
   const int64_t record = page * a.cache.kv_heads + h;
-  uint8_t* const keys = a.cache.key + record * kPage * kDim;
-  uint8_t* const values = a.cache.value + record * kPage * kDim;
+  uint8_t* const keys = a.cache.key + record * (kPage * kDim);
+  uint8_t* const values = a.cache.value + record * (kPage * kDim);
   const bool fills = in.slot + in.n == kPage;
-  float upper[kPer], lower[kPer];
-  for (int e = 0; e < kPer; ++e) upper[e] = -__builtin_inff(), lower[e] = __builtin_inff();
+  const int begin = fills ? 0 : in.slot / 8, end = (in.slot + in.n + 7) / 8;
+  const uint16_t* const key_rows = static_cast<const uint16_t*>(a.key.data) + b * a.key.stride_batch + h * a.key.stride_head + E::kValues * c;
+  const uint16_t* const value_rows = static_cast<const uint16_t*>(a.value.data) + b * a.value.stride_batch + h * a.value.stride_head + E::kValues * c;
+  float upper[E::kValues], lower[E::kValues];
+#pragma unroll
+  for (int i = 0; i < E::kValues; ++i) upper[i] = -__builtin_inff(), lower[i] = __builtin_inff();
 
-  for (int slot = fills ? 0 : in.slot; slot < in.slot + in.n; ++slot) {
-    float k[kPer];
-    if (slot < in.slot) {  // a full page's earlier keys, for its bounds
-      const float s = a.cache.key_scale[record * kPage + slot];
-      for (int e = 0; e < kPer; ++e) k[e] = code_value<kFp8>(keys[slot * kDim + lane * kPer + e]) * s;
-    } else {
-      const int64_t i = in.first + slot - in.slot;
-      for (int part = 0; part < 2; ++part) {
-        const InputTensor& t = part == 0 ? a.key : a.value;
-        const uint16_t* row = static_cast<const uint16_t*>(t.data) + b * t.stride_batch + h * t.stride_head + i * t.stride_seq;
-        float x[kPer], top = 0.0f;
-        bool finite = true;
-        for (int e = 0; e < kPer; ++e) {
-          x[e] = widen<kBf16>(row[lane * kPer + e]);
-          top = fmaxf(top, fabsf(x[e]));
-          finite = finite && is_finite(x[e]);
-        }
-        const RowCode code = row_code<kFp8>(wave_max(top), __all(finite));
-        for (int e = 0; e < kPer; ++e) {
-          const uint32_t c = code_of_value<kFp8>(x[e], code.inv);
-          if (part == 0) {
-            keys[slot * kDim + lane * kPer + e] = static_cast<uint8_t>(c);
-            k[e] = code_value<kFp8>(c) * code.scale;
-          } else {
-            values[value_offset(slot, lane * kPer + e, kDim)] = static_cast<uint8_t>(c);
-          }
-        }
-        if (lane == 0) (part == 0 ? a.cache.key_scale : a.cache.value_scale)[record * kPage + slot] = code.scale;
+  for (int eight = begin + wave; eight < end; eight += kMoveWaves) {
+    const int slot = 8 * eight + r;
+    const bool mine = slot >= in.slot && slot < in.slot + in.n;  // a row of the call
+    const int64_t row = in.first + (mine ? slot - in.slot : 0);
+    uint4 key[E::kLoads], value[E::kLoads];
+#pragma unroll
+    for (int k = 0; k < E::kLoads; ++k) {
+      key[k] = *reinterpret_cast<const uint4*>(key_rows + row * a.key.stride_seq + 8 * k);
+      value[k] = *reinterpret_cast<const uint4*>(value_rows + row * a.value.stride_seq + 8 * k);
+    }
+    uint32_t codes[E::kWords], tokens[E::kWords];
+    float scale = encode_row<kBf16, kFp8, kDim>(value, codes);
+    tokens_together<kDim>(codes, tokens, r);
+    uint8_t* const to = values + eight * (8 * kDim) + (8 * c + r) * kDim / 8;
+    if (8 * eight >= in.slot && 8 * eight + 8 <= in.slot + in.n) {
+      if constexpr (kDim == 128)
+        *reinterpret_cast<uint4*>(to) = uint4{tokens[0], tokens[1], tokens[2], tokens[3]};
+      else
+        *reinterpret_cast<uint2*>(to) = uint2{tokens[0], tokens[1]};
+    } else {  // the other slots' bytes stay
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        if (8 * eight + t < in.slot || 8 * eight + t >= in.slot + in.n) continue;
+#pragma unroll
+        for (int f = 0; f < kDim / 64; ++f) to[8 * f + t] = static_cast<uint8_t>(tokens[2 * f + t / 4] >> (8 * (t % 4)));
       }
     }
-    for (int e = 0; e < kPer; ++e) upper[e] = fmaxf(upper[e], k[e]), lower[e] = fminf(lower[e], k[e]);
-  }
-  if (!fills) return;
-  float top = 0.0f;
-  for (int e = 0; e < kPer; ++e) {
-    if (upper[e] < lower[e]) upper[e] = lower[e] = 0.0f;  // every key of the page is NaN
-    top = fmaxf(top, fmaxf(fabsf(upper[e]), fabsf(lower[e])));
-  }
-  const RowCode code = row_code<false>(wave_max(top), true);
-  for (int e = 0; e < kPer; ++e) {
-    a.cache.bounds[record * 2 * kDim + lane * kPer + e] = static_cast<int8_t>(code_of_value<false>(upper[e], code.inv));
-    a.cache.bounds[record * 2 * kDim + kDim + lane * kPer + e] = static_cast<int8_t>(code_of_value<false>(lower[e], code.inv));
-  }
-  if (lane == 0) a.cache.bound_scale[record] = code.scale;
-}
-
-// ---- read -----------------------------------------------------------------------------------------------------------
-
-// One thread per eight features of a row's key and value.
-template <bool kBf16, bool kFp8, int kDim>
-__global__ __launch_bounds__(256) void cache_read_kernel(CacheMove a) {
-  constexpr int kPieces = kDim / 8;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t row = at / kPieces;
-  const int piece = static_cast<int>(at % kPieces);
-  const int64_t i = row % a.rows.tokens, unit = row / a.rows.tokens;
-  const int64_t b = unit / a.cache.kv_heads, h = unit % a.cache.kv_heads;
-  if (b >= a.batch) return;
-  const int64_t position = a.rows.start(b) + i;
-  const int64_t page = i < a.rows.count(b) && position >= 0 ? a.rows.page(b, position / kPage) : -1;
-  uint32_t key[4] = {}, value[4] = {};
-  if (page >= 0) {
-    const int64_t record = page * a.cache.kv_heads + h;
-    const int slot = static_cast<int>(position % kPage);
-    const float ks = a.cache.key_scale[record * kPage + slot], vs = a.cache.value_scale[record * kPage + slot];
-    const uint8_t* k = a.cache.key + record * kPage * kDim + slot * kDim + piece * 8;
-    const uint8_t* v = a.cache.value + record * kPage * kDim + value_offset(slot, piece * 8, kDim);
-    for (int e = 0; e < 4; ++e) {
-      key[e] = narrow2<kBf16>(code_value<kFp8>(k[2 * e]) * ks, code_value<kFp8>(k[2 * e + 1]) * ks);
-      value[e] = narrow2<kBf16>(code_value<kFp8>(v[16 * e]) * vs, code_value<kFp8>(v[16 * e + 8]) * vs);
+    if (mine && c == 0) a.cache.value_scale[record * kPage + slot] = scale;
+    scale = encode_row<kBf16, kFp8, kDim>(key, codes);
+    uint8_t* const key_to = keys + slot * kDim + E::kValues * c;
+    if (mine) {
+      if constexpr (kDim == 128)
+        *reinterpret_cast<uint4*>(key_to) = uint4{codes[0], codes[1], codes[2], codes[3]};
+      else
+        *reinterpret_cast<uint2*>(key_to) = uint2{codes[0], codes[1]};
+      if (c == 0) a.cache.key_scale[record * kPage + slot] = scale;
+    } else if (fills) {  // a full page's earlier keys, for its bounds
+      scale = a.cache.key_scale[record * kPage + slot];
+#pragma unroll
+      for (int w = 0; w < E::kWords; ++w) codes[w] = reinterpret_cast<const uint32_t*>(key_to)[w];
+    }
+    if (fills) {
+#pragma unroll
+      for (int w = 0; w < E::kWords; ++w) {
+        float x[4];
+        decode4<kFp8>(codes[w], x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float k = x[i] * scale;  // NaN is left out
+          upper[4 * w + i] = fmaxf(upper[4 * w + i], k);
+          lower[4 * w + i] = fminf(lower[4 * w + i], k);
+        }
+      }
     }
   }
-  const_cast<uint4*>(static_cast<const uint4*>(a.key.data))[at] = uint4{key[0], key[1], key[2], key[3]};
-  const_cast<uint4*>(static_cast<const uint4*>(a.value.data))[at] = uint4{value[0], value[1], value[2], value[3]};
+  if (!fills) return;
+#pragma unroll
+  for (int i = 0; i < E::kValues; ++i) {  // over a wave's tokens: lanes 8, 16 and 32 apart
+    upper[i] = fmaxf(upper[i], __uint_as_float(lane_xor8(__float_as_uint(upper[i]))));
+    lower[i] = fminf(lower[i], __uint_as_float(lane_xor8(__float_as_uint(lower[i]))));
+    uint32_t u = __float_as_uint(upper[i]), v = __float_as_uint(upper[i]);
+    exchange16(u, v);
+    upper[i] = fmaxf(__uint_as_float(u), __uint_as_float(v));
+    u = v = __float_as_uint(upper[i]);
+    exchange32(u, v);
+    upper[i] = fmaxf(__uint_as_float(u), __uint_as_float(v));
+    u = v = __float_as_uint(lower[i]);
+    exchange16(u, v);
+    lower[i] = fminf(__uint_as_float(u), __uint_as_float(v));
+    u = v = __float_as_uint(lower[i]);
+    exchange32(u, v);
+    lower[i] = fminf(__uint_as_float(u), __uint_as_float(v));
+    if (r == 0) {
+      ends[wave][0][E::kValues * c + i] = upper[i];
+      ends[wave][1][E::kValues * c + i] = lower[i];
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < kDim) {
+    float up = ends[0][0][threadIdx.x], low = ends[0][1][threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < kMoveWaves; ++w) up = fmaxf(up, ends[w][0][threadIdx.x]), low = fminf(low, ends[w][1][threadIdx.x]);
+    if (up < low) up = low = 0.0f;  // every key of the page is NaN
+    ends[0][0][threadIdx.x] = up;
+    ends[0][1][threadIdx.x] = low;
+    const float top = wave_max(fmaxf(fabsf(up), fabsf(low)));
+    if (lane == 0) tops[wave] = top;
+  }
+  __syncthreads();
+  if (threadIdx.x < kDim) {
+    const RowCode code = row_code<false>(kDim == 128 ? fmaxf(tops[0], tops[1]) : tops[0], true);
+    int8_t* const to = a.cache.bounds + record * 2 * kDim + threadIdx.x;
+    to[0] = static_cast<int8_t>(code_of_value<false>(ends[0][0][threadIdx.x], code.inv));
+    to[kDim] = static_cast<int8_t>(code_of_value<false>(ends[0][1][threadIdx.x], code.inv));
+    if (threadIdx.x == 0) a.cache.bound_scale[record] = code.scale;
+  }
+}
+
+template <bool kBf16, bool kFp8>
+__device__ __forceinline__ uint2 decode_row4(uint32_t codes, float scale) {
+  float x[4];
+  decode4<kFp8>(codes, x);
+  return uint2{narrow2<kBf16>(x[0] * scale, x[1] * scale), narrow2<kBf16>(x[2] * scale, x[3] * scale)};
+}
+
+// Values of the rows of a page of one K/V head, and zeros for those of them that are padding or have no page.
+template <bool kBf16, bool kFp8, int kDim>
+__global__ __launch_bounds__(kWave* kMoveWaves) void cache_read_kernel(CacheMove a) {
+  using E = Eighth<kDim>;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r = lane / 8, c = lane % 8;
+  const int64_t touched = pages_touched(a.rows.tokens);
+  const int64_t unit = blockIdx.x / touched;
+  const int64_t b = unit / a.cache.kv_heads, h = unit % a.cache.kv_heads;
+  const int64_t start = a.rows.start(b), logical = floor_page(start) + blockIdx.x % touched, base = logical * kPage;
+  const int count = a.rows.count(b);
+  const int64_t page = a.rows.page(b, logical);
+  const int64_t record = (page >= 0 ? page : 0) * a.cache.kv_heads + h;
+  uint16_t* const key_out = static_cast<uint16_t*>(const_cast<void*>(a.key.data)) + unit * a.rows.tokens * kDim;
+  uint16_t* const value_out = static_cast<uint16_t*>(const_cast<void*>(a.value.data)) + unit * a.rows.tokens * kDim;
+  const uint8_t* const keys = a.cache.key + record * (kPage * kDim);
+  const uint8_t* const values = a.cache.value + record * (kPage * kDim);
+#pragma unroll
+  for (int k = 0; k < 8 / kMoveWaves; ++k) {
+    const int eight = wave + k * kMoveWaves;
+    // rows base - start + slot of the call, of which [0, tokens) exist
+    const int64_t first = base - start + 8 * eight;
+    if (first + 8 <= 0 || first >= a.rows.tokens) continue;
+    {
+      const int slot = 8 * eight + r;
+      const int64_t row = first + r;
+      const float held = a.cache.key_scale[record * kPage + slot];
+      uint32_t codes[E::kWords];
+#pragma unroll
+      for (int w = 0; w < E::kWords; ++w) codes[w] = reinterpret_cast<const uint32_t*>(keys + slot * kDim + E::kValues * c)[w];
+      const bool real = page >= 0 && row < count;
+      if (row >= 0 && row < a.rows.tokens) {
+#pragma unroll
+        for (int w = 0; w < E::kWords; w += 2) {
+          const uint2 x = decode_row4<kBf16, kFp8>(codes[w], held), y = decode_row4<kBf16, kFp8>(codes[w + 1], held);
+          *reinterpret_cast<uint4*>(key_out + row * kDim + E::kValues * c + 4 * w) = real ? uint4{x.x, x.y, y.x, y.y} : uint4{0, 0, 0, 0};
+        }
+      }
+    }
+    // values: a lane's eight tokens of features 2 lane and 2 lane + 1, or of feature lane
+    uint32_t codes[E::kWords];
+#pragma unroll
+    for (int w = 0; w < E::kWords; ++w) codes[w] = reinterpret_cast<const uint32_t*>(values + eight * (8 * kDim) + lane * (kDim / 8))[w];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const float4 held = *reinterpret_cast<const float4*>(a.cache.value_scale + record * kPage + 8 * eight + 4 * half);
+      const float scale[4] = {held.x, held.y, held.z, held.w};
+      float x[4], y[4] = {};
+      decode4<kFp8>(codes[half], x);
+      if constexpr (kDim == 128) decode4<kFp8>(codes[2 + half], y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t row = first + 4 * half + i;
+        if (row < 0 || row >= a.rows.tokens) continue;
+        const uint32_t packed = page >= 0 && row < count ? narrow2<kBf16>(x[i] * scale[i], y[i] * scale[i]) : 0u;
+        if constexpr (kDim == 128)
+          reinterpret_cast<uint32_t*>(value_out + row * kDim)[lane] = packed;
+        else
+          value_out[row * kDim + lane] = static_cast<uint16_t>(packed);
+      }
+    }
+  }
 }
 
 // ---- selection ------------------------------------------------------------------------------------------------------
@@ -458,20 +693,23 @@ __global__ __launch_bounds__(kWave* kSelectWaves) void cache_pick_kernel(CacheSe
 
 }  // namespace
 
+// A workgroup for each page that a sequence's rows can touch.
+static dim3 move_blocks(const CacheMove& a) {
+  return dim3(static_cast<uint32_t>(static_cast<int64_t>(a.batch) * a.cache.kv_heads * pages_touched(a.rows.tokens)));
+}
+
 hipError_t launch_cache_write(const CacheMove& a, CacheForm form, hipStream_t stream) {
-  const int64_t blocks = a.batch * a.cache.kv_heads * pages_touched(a.rows.tokens);
   return with_cache_form(form, [&](auto bf16, auto fp8, auto dim) {
     cache_write_kernel<decltype(bf16)::value, decltype(fp8)::value, decltype(dim)::value>
-        <<<dim3(static_cast<uint32_t>(blocks)), dim3(kWave), 0, stream>>>(a);
+        <<<move_blocks(a), dim3(kWave * kMoveWaves), 0, stream>>>(a);
     return hipGetLastError();
   });
 }
 
 hipError_t launch_cache_read(const CacheMove& a, CacheForm form, hipStream_t stream) {
-  const int64_t threads = static_cast<int64_t>(a.batch) * a.cache.kv_heads * a.rows.tokens * (form.head_dim / 8);
   return with_cache_form(form, [&](auto bf16, auto fp8, auto dim) {
     cache_read_kernel<decltype(bf16)::value, decltype(fp8)::value, decltype(dim)::value>
-        <<<dim3(static_cast<uint32_t>(ceil_div(threads, 256))), dim3(256), 0, stream>>>(a);
+        <<<move_blocks(a), dim3(kWave * kMoveWaves), 0, stream>>>(a);
     return hipGetLastError();
   });
 }
