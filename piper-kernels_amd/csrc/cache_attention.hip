@@ -570,6 +570,20 @@ struct TileShared {
   float key_scale[2][kPage], value_scale[2][kPage];  // the values' in units of 2^-15 of the reference
 };
 
+// The order of a block of kReads LDS reads that feed as many matrix instructions: six reads ahead, or the scheduler, to
+// save registers, waits for each pair's.
+template <int kReads>
+__device__ __forceinline__ void reads_ahead() {
+  constexpr int kDsRead = 0x100, kMatrix = 0x8, kAhead = 6;
+  __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
+#pragma unroll
+  for (int i = kAhead; i < kReads; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(kMatrix, kAhead, 0);
+}
+
 template <bool kBf16, bool kFp8, int kDim, int kTileWaves>
 struct Tile {
   static constexpr int kSteps = kDim / 16, kFeatures = kDim / 32;
@@ -662,29 +676,46 @@ struct Tile {
   __device__ __forceinline__ void use(int buffer, float unit, uint32_t seen) {
     float16_t score[2];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) score[kt][i] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k)
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
         score[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(shared.key[buffer][32 * kt + n][(2 * k + g) ^ (n & 7)], query[k], score[kt], 0, 0, 0);
-    }
+    reads_ahead<2 * kSteps>();
+    // eight keys' scales stand together; read ahead of their use, which the scheduler would put off to save registers
+    float4 scales[2][2][2];
+    const auto read = [&](const float (&from)[kPage]) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) scales[kt][p][q] = *reinterpret_cast<const float4*>(&from[32 * kt + 16 * p + 8 * g + 4 * q]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    read(shared.key_scale[buffer]);
     float page_top = kNone;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int first = 32 * kt + 16 * (q / 2) + 8 * g + 4 * (q % 2);
-        const float4 s = *reinterpret_cast<const float4*>(&shared.key_scale[buffer][first]);
-        const float ks[4] = {s.x, s.y, s.z, s.w};
+      for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = score[kt][4 * q + i] * ks[i];
-          if constexpr (kMasked) x = seen >> (16 * kt + 4 * q + i) & 1 ? x : kNone;
-          score[kt][4 * q + i] = x;
-          page_top = fmaxf(page_top, x);
+        for (int q = 0; q < 2; ++q) {
+          const float4 s = scales[kt][p][q];
+          const float ks[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = 8 * p + 4 * q + i;
+            float x = score[kt][at] * ks[i];
+            if constexpr (kMasked) x = seen >> (16 * kt + at) & 1 ? x : kNone;
+            score[kt][at] = x;
+            page_top = fmaxf(page_top, x);
+          }
         }
-      }
+    read(shared.value_scale[buffer]);
     const float next = fmaxf(top, cross_half_max(page_top) * factor);
     const float base = next == kNone ? 0.0f : next;
     const float keep = exp2_fast(top - base);
@@ -694,10 +725,11 @@ struct Tile {
       for (int f = 0; f < kFeatures; ++f)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum[f][i] *= scale;
+      total *= keep;
     }
     top = next;
     sum_reference = unit;
-    total *= keep;
+    half8 weight[2][2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -705,7 +737,7 @@ struct Tile {
         uint32_t packed[4];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const float4 s = *reinterpret_cast<const float4*>(&shared.value_scale[buffer][32 * kt + 16 * p + 8 * g + 4 * q]);
+          const float4 s = scales[kt][p][q];
           const float vs[4] = {s.x, s.y, s.z, s.w};
           float w[4];
 #pragma unroll
@@ -719,11 +751,17 @@ struct Tile {
           packed[2 * q] = pack_half2(w[0], w[1]);
           packed[2 * q + 1] = pack_half2(w[2], w[3]);
         }
-        const half8 weight = __builtin_bit_cast(half8, uint4{packed[0], packed[1], packed[2], packed[3]});
+        weight[kt][p] = __builtin_bit_cast(half8, uint4{packed[0], packed[1], packed[2], packed[3]});
+      }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int f = 0; f < kFeatures; ++f)
-          sum[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(shared.value[buffer][4 * kt + 2 * p + g][32 * f + n], weight, sum[f], 0, 0, 0);
-      }
+          sum[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(shared.value[buffer][4 * kt + 2 * p + g][32 * f + n], weight[kt][p], sum[f], 0, 0, 0);
+    reads_ahead<4 * kFeatures>();
   }
 };
 
