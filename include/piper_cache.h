@@ -9,7 +9,7 @@
  * share buffers.
  *
  * The cache.  A page holds 64 tokens (PIPER_CACHE_PAGE) of every K/V head.  With P pages, H K/V heads and
- * head size D all arrays are dense and row-major, each 16-byte aligned:
+ * head size D all arrays are dense and row-major, each 16-byte aligned (bound_scale: 4-byte):
  *
  *   key          8 bit  [P, H, 64, D]
  *   key_scale    float  [P, H, 64]
@@ -30,6 +30,10 @@
  * sequence b, i < counts[b] (NULL: every row), is position starts[b] + i.  All three live in device memory.
  * Positions below 0 or beyond the table and entries outside [0, P) name no page: nothing is written there, reads
  * give zeros and attention does not see it.  Counts are taken as 0 below 0 and as the row count beyond it.
+ *
+ * A call that would take 2^23 workgroups or more is refused (PIPER_ERROR_UNSUPPORTED).  Workgroups: for a write or a read one
+ * per page touched and K/V head; for attention one per K/V head and block of up to 16, 32, 128 or 256 query rows
+ * (with selected pages one per token and up to 32); for selection at most one per row, K/V head and 256 pages.
  */
 #ifndef PIPER_CACHE_H
 #define PIPER_CACHE_H
@@ -145,7 +149,8 @@ int piper_cache_attention_workspace_bytes(const piper_cache_attention_args* args
  * c_h and scale s_h by the cache's rule, a page's score is
  *     max over the K/V head's query heads of (sum_d max(c_h[d], 0) upper[d] + min(c_h[d], 0) lower[d]) * s_h,  times bound_scale:
  * the sum in integers, both products in FP32, so every order of evaluation gives the same score.  A page that the
- * table does not name has score -inf.  Rows >= counts[b], and rows whose position the table does not reach, are
+ * table does not name has score -inf.  Heads whose query row is not finite are left out of the maximum; where all
+ * are, every page has score -inf.  Rows >= counts[b], and rows whose position the table does not reach, are
  * all -1. */
 int piper_cache_select(const piper_cache_select_args* args, void* stream);
 int piper_cache_select_workspace_bytes(const piper_cache_select_args* args, int64_t* bytes);

@@ -272,11 +272,21 @@ __global__ __launch_bounds__(kWave* kMoveWaves) void cache_write_kernel(CacheMov
   }
 }
 
+// Two values' products in FP32, then the output's rounding. For FP16 the compiler would make one instruction of the
+// two (v_fma_mixlo_f16, one rounding, whatever the contraction mode), and a few values would differ by an ulp from
+// what the cache is defined to hold: the products are pinned in registers between.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t narrow_product2(float x, float y, float scale) {
+  float a = x * scale, b = y * scale;
+  if constexpr (!kBf16) asm("" : "+v"(a), "+v"(b));
+  return narrow2<kBf16>(a, b);
+}
+
 template <bool kBf16, bool kFp8>
 __device__ __forceinline__ uint2 decode_row4(uint32_t codes, float scale) {
   float x[4];
   decode4<kFp8>(codes, x);
-  return uint2{narrow2<kBf16>(x[0] * scale, x[1] * scale), narrow2<kBf16>(x[2] * scale, x[3] * scale)};
+  return uint2{narrow_product2<kBf16>(x[0], x[1], scale), narrow_product2<kBf16>(x[2], x[3], scale)};
 }
 
 // Values of the rows of a page of one K/V head, and zeros for those of them that are padding or have no page.
@@ -332,7 +342,7 @@ __global__ __launch_bounds__(kWave* kMoveWaves) void cache_read_kernel(CacheMove
       for (int i = 0; i < 4; ++i) {
         const int64_t row = first + 4 * half + i;
         if (row < 0 || row >= a.rows.tokens) continue;
-        const uint32_t packed = page >= 0 && row < count ? narrow2<kBf16>(x[i] * scale[i], y[i] * scale[i]) : 0u;
+        const uint32_t packed = page >= 0 && row < count ? narrow_product2<kBf16>(x[i], y[i], scale[i]) : 0u;
         if constexpr (kDim == 128)
           reinterpret_cast<uint32_t*>(value_out + row * kDim)[lane] = packed;
         else
@@ -357,9 +367,10 @@ constexpr int kSelectWaves = 8;
 constexpr int kRowScores = 16384;  // scores in LDS: 64 KiB, two workgroups a CU; also what a workgroup's registers hold
 constexpr int kWaveScores = 1024;  // what one wave's registers hold
 
-// Scores in the order of whole numbers: the larger the score, the larger the number (-0 is 0); all of them above 0.
+// Scores in the order of whole numbers: the larger the score, the larger the number (-0 is 0, NaN -infinity); all of
+// them above 0, which stands for no score.
 __device__ __forceinline__ uint32_t score_order(float score) {
-  const uint32_t u = __float_as_uint(score + 0.0f);
+  const uint32_t u = __float_as_uint(fmaxf(score, -__builtin_inff()) + 0.0f);
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
@@ -737,24 +748,31 @@ int64_t cache_select_scores(const CacheSelect& a, int cus) {
   return select_tokens(a, cus) > 0 ? 0 : static_cast<int64_t>(a.batch) * a.cache.kv_heads * a.rows.tokens * a.rows.table_width;
 }
 
-hipError_t launch_cache_select(const CacheSelect& a, CacheForm form, int cus, hipStream_t stream) {
+// Workgroups for a row's scores in the workspace.
+static int score_parts(const CacheSelect& a) { return static_cast<int>(ceil_div(a.rows.table_width, 4 * kScoreTiles * 16)); }
+
+int64_t cache_select_workgroups(const CacheSelect& a, int cus) {
   const int64_t units = static_cast<int64_t>(a.batch) * a.cache.kv_heads;
+  const int tokens = select_tokens(a, cus);
+  return tokens > 0 ? units * ceil_div(a.rows.tokens, tokens) : units * a.rows.tokens * score_parts(a);
+}
+
+hipError_t launch_cache_select(const CacheSelect& a, CacheForm form, int cus, hipStream_t stream) {
   const int tokens = select_tokens(a, cus), columns = select_columns(a);
+  const dim3 blocks(static_cast<uint32_t>(cache_select_workgroups(a, cus)));
   form.fp8 = false;  // the bounds are INT8 in every cache
   return with_cache_form(form, [&](auto bf16, auto, auto dim) {
     constexpr bool kBf16 = decltype(bf16)::value;
     constexpr int kDim = decltype(dim)::value;
     if (tokens > 0) {
-      const int64_t blocks = units * ceil_div(a.rows.tokens, tokens);
-      cache_select_kernel<kBf16, kDim><<<dim3(static_cast<uint32_t>(blocks)), dim3(kWave * kSelectWaves),
-                                         static_cast<size_t>(tokens) * a.rows.table_width * 4, stream>>>(a, tokens, columns);
+      cache_select_kernel<kBf16, kDim><<<blocks, dim3(kWave * kSelectWaves), static_cast<size_t>(tokens) * a.rows.table_width * 4, stream>>>(
+          a, tokens, columns);
       return hipGetLastError();
     }
-    const int parts = static_cast<int>(ceil_div(a.rows.table_width, 4 * kScoreTiles * 16));
-    const int64_t rows = units * a.rows.tokens;
-    cache_score_kernel<kBf16, kDim><<<dim3(static_cast<uint32_t>(rows * parts)), dim3(256), 0, stream>>>(a, columns, parts);
+    const int parts = score_parts(a);
+    cache_score_kernel<kBf16, kDim><<<blocks, dim3(256), 0, stream>>>(a, columns, parts);
     if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
-    cache_pick_kernel<<<dim3(static_cast<uint32_t>(rows)), dim3(kWave * kSelectWaves), 0, stream>>>(a);
+    cache_pick_kernel<<<dim3(blocks.x / parts), dim3(kWave * kSelectWaves), 0, stream>>>(a);
     return hipGetLastError();
   });
 }
@@ -768,7 +786,8 @@ namespace {
 using piper::aligned16;
 using piper::fail;
 
-constexpr int64_t kMaxBlocks = int64_t(1) << 30;  // of a launch; grids are 32-bit
+constexpr int64_t kMaxRows = int64_t(1) << 30;  // of a call, times its heads
+constexpr int kMaxThreads = 512;                // of a workgroup of these kernels
 
 int check_version(int32_t version) {
   if (version != PIPER_CACHE_ABI_VERSION)
@@ -789,12 +808,21 @@ int check_sizes(const piper_cache& c, const piper_cache_rows& r) {
   if (c.pages <= 0 || c.kv_heads <= 0 || r.batch <= 0 || r.tokens <= 0 || r.table_width <= 0)
     return fail(PIPER_ERROR_INVALID_ARGUMENT, "sizes must be positive, got pages=%lld kv_heads=%lld batch=%lld tokens=%lld table_width=%lld",
                 (long long)c.pages, (long long)c.kv_heads, (long long)r.batch, (long long)r.tokens, (long long)r.table_width);
-  // pages and widths are int32 in the kernels, as table entries are; a grid has at most kMaxBlocks workgroups
+  // pages and widths are int32 in the kernels, as table entries are
   if (c.pages > INT32_MAX || r.table_width > (1 << 24) || r.tokens > (1 << 26) || c.kv_heads > (1 << 16) || r.batch > (1 << 24) ||
-      r.batch * c.kv_heads > kMaxBlocks / r.tokens)
+      r.batch * c.kv_heads > kMaxRows / r.tokens)
     return fail(PIPER_ERROR_UNSUPPORTED, "cache call too large for this build");
   return PIPER_OK;
 }
+
+// A launch's threads are counted in 32 bits.
+int check_launch(int64_t workgroups) {
+  if (workgroups > UINT32_MAX / kMaxThreads) return fail(PIPER_ERROR_UNSUPPORTED, "cache call too large for this build");
+  return PIPER_OK;
+}
+
+// Workgroups of a write or a read.
+int64_t move_workgroups(const piper_cache& c, const piper_cache_rows& r) { return r.batch * c.kv_heads * piper::pages_touched(r.tokens); }
 
 int check_rows(const piper_cache_rows& r) {
   if (r.page_table == nullptr || r.starts == nullptr) return fail(PIPER_ERROR_INVALID_ARGUMENT, "page_table or starts is NULL");
@@ -811,7 +839,8 @@ int check_codes(const piper_cache& c) {
 
 int check_bounds(const piper_cache& c) {
   if (!c.bounds || !c.bound_scale) return fail(PIPER_ERROR_INVALID_ARGUMENT, "a cache pointer is NULL");
-  if (!aligned16(c.bounds) || !aligned16(c.bound_scale)) return fail(PIPER_ERROR_INVALID_ARGUMENT, "cache arrays must be 16-byte aligned");
+  if (!aligned16(c.bounds)) return fail(PIPER_ERROR_INVALID_ARGUMENT, "cache arrays must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(c.bound_scale) % 4 != 0) return fail(PIPER_ERROR_INVALID_ARGUMENT, "bound_scale must be 4-byte aligned");
   return PIPER_OK;
 }
 
@@ -832,7 +861,7 @@ int check_heads(int64_t heads, const piper_cache& c, const piper_cache_rows& r) 
   if (heads <= 0 || heads % c.kv_heads != 0)
     return fail(PIPER_ERROR_INVALID_ARGUMENT, "heads must be a positive multiple of kv_heads, got %lld and %lld", (long long)heads,
                 (long long)c.kv_heads);
-  if (heads > (1 << 20) || r.batch * heads > kMaxBlocks / r.tokens) return fail(PIPER_ERROR_UNSUPPORTED, "cache call too large for this build");
+  if (heads > (1 << 20) || r.batch * heads > kMaxRows / r.tokens) return fail(PIPER_ERROR_UNSUPPORTED, "cache call too large for this build");
   return PIPER_OK;
 }
 
@@ -910,6 +939,7 @@ extern "C" int piper_cache_write(const piper_cache_write_args* a, void* stream) 
   if (int st = check_version(a->abi_version)) return st;
   if (int st = check_dtype(a->dtype)) return st;
   if (int st = check_sizes(a->cache, a->rows)) return st;
+  if (int st = check_launch(move_workgroups(a->cache, a->rows))) return st;
   if (int st = check_rows(a->rows)) return st;
   if (int st = check_codes(a->cache)) return st;
   if (int st = check_bounds(a->cache)) return st;
@@ -925,6 +955,7 @@ extern "C" int piper_cache_read(const piper_cache_read_args* a, void* stream) {
   if (int st = check_version(a->abi_version)) return st;
   if (int st = check_dtype(a->dtype)) return st;
   if (int st = check_sizes(a->cache, a->rows)) return st;
+  if (int st = check_launch(move_workgroups(a->cache, a->rows))) return st;
   if (int st = check_rows(a->rows)) return st;
   if (int st = check_codes(a->cache)) return st;
   if (int st = check_output("key", a->key)) return st;
@@ -939,7 +970,9 @@ extern "C" int piper_cache_attention_workspace_bytes(const piper_cache_attention
   if (int st = check_attention(a)) return st;
   int cus = 0, xccs = 0;
   if (int st = piper::device_topology(&cus, &xccs)) return st;
-  *bytes = piper::cache_attention_parts(attention_of(*a), a->cache.head_dim, cus).bytes;
+  const piper::CacheParts parts = piper::cache_attention_parts(attention_of(*a), a->cache.head_dim, cus);
+  if (int st = check_launch(parts.workgroups)) return st;
+  *bytes = parts.bytes;
   return PIPER_OK;
 }
 
@@ -956,7 +989,7 @@ extern "C" int piper_cache_attention(const piper_cache_attention_args* a, void* 
   if (int st = piper::device_topology(&cus, &xccs)) return st;
   piper::CacheAttention attention = attention_of(*a);
   const piper::CacheParts parts = piper::cache_attention_parts(attention, a->cache.head_dim, cus);
-  if (parts.workgroups > kMaxBlocks) return fail(PIPER_ERROR_UNSUPPORTED, "cache call too large for this build");
+  if (int st = check_launch(parts.workgroups)) return st;  // more than there are to join
   if (int st = check_workspace(a->workspace, a->workspace_bytes, parts.bytes)) return st;
   attention.shares = parts.shares;
   attention.parts = static_cast<int32_t>(parts.parts);
@@ -975,7 +1008,9 @@ extern "C" int piper_cache_select_workspace_bytes(const piper_cache_select_args*
   if (int st = check_select(a)) return st;
   int cus = 0, xccs = 0;
   if (int st = piper::device_topology(&cus, &xccs)) return st;
-  *bytes = 4 * piper::cache_select_scores(select_of(*a), cus);
+  const piper::CacheSelect select = select_of(*a);
+  if (int st = check_launch(piper::cache_select_workgroups(select, cus))) return st;
+  *bytes = 4 * piper::cache_select_scores(select, cus);
   return PIPER_OK;
 }
 
@@ -988,10 +1023,7 @@ extern "C" int piper_cache_select(const piper_cache_select_args* a, void* stream
   const piper::CacheSelect select = select_of(*a);
   int cus = 0, xccs = 0;
   if (int st = piper::device_topology(&cus, &xccs)) return st;
-  const int64_t scores = piper::cache_select_scores(select, cus);
-  // the score kernel has a workgroup for each 256 pages of a row
-  if (scores / 256 + a->rows.batch * a->heads * a->rows.tokens > kMaxBlocks)
-    return fail(PIPER_ERROR_UNSUPPORTED, "cache call too large for this build");
-  if (int st = check_workspace(a->workspace, a->workspace_bytes, 4 * scores)) return st;
+  if (int st = check_launch(piper::cache_select_workgroups(select, cus))) return st;
+  if (int st = check_workspace(a->workspace, a->workspace_bytes, 4 * piper::cache_select_scores(select, cus))) return st;
   return launched(piper::launch_cache_select(select, form_of(a->cache, a->dtype), cus, static_cast<hipStream_t>(stream)), "cache select");
 }

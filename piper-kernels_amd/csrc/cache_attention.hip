@@ -127,7 +127,7 @@ __device__ __forceinline__ void walk_line(const CacheAttention& a, int block_row
   const int64_t end = at + share < total ? at + share : total;
   if (at < end) {
     int found = 0;
-    for (int64_t b0 = 0; found == 0; b0 += kWave) {
+    for (int64_t b0 = 0; found == 0 && b0 < a.batch; b0 += kWave) {
       const int mine = b0 == 0 ? length0 : length(b0 + lane), prefix = b0 == 0 ? prefix0 : wave_prefix(mine);
       const uint64_t holds = __ballot(first + static_cast<int64_t>(prefix) * heads > at);
       if (holds != 0) {
@@ -139,6 +139,7 @@ __device__ __forceinline__ void walk_line(const CacheAttention& a, int block_row
         first += static_cast<int64_t>(__builtin_amdgcn_readlane(prefix, kWave - 1)) * heads;
       }
     }
+    if (found == 0) return;  // starts or counts changed under the kernel
     int n = pages_of<false>(a, b), blocks = blocks_of(b);
     int block = static_cast<int>((at - first) / n);
     int lo = static_cast<int>((at - first) % n);
@@ -157,8 +158,10 @@ __device__ __forceinline__ void walk_line(const CacheAttention& a, int block_row
         block = 0;
         if (++h == heads) {
           h = 0;
-          do n = pages_of<false>(a, ++b), blocks = blocks_of(b);
-          while (n * blocks == 0);  // the line is not at its end: a sequence with rows and pages follows
+          do {  // the line is not at its end: a sequence with rows and pages follows
+            if (++b >= a.batch) return;
+            n = pages_of<false>(a, b), blocks = blocks_of(b);
+          } while (n == 0 || blocks == 0);
         }
       }
       __syncthreads();
@@ -997,6 +1000,7 @@ CacheParts cache_attention_parts(const CacheAttention& a, int head_dim, int cus)
   } else {
     const int64_t slots = static_cast<int64_t>(cus) * (rows == 256 ? 1 : 2);
     if (blocks >= 8 * slots) return p;
+    if (pages * p.blocks_of_unit > INT32_MAX / kWave) return p;  // walk_line adds a wave's lengths in 32 bits
     p.shares = CacheShares::kLine;
     p.workgroups = std::min(slots, ceil_div(blocks * pages, p.least_share));
     p.rows = (blocks + p.workgroups) * rows;

@@ -72,7 +72,8 @@ struct CacheForm {
   int head_dim;
 };
 
-int64_t cache_select_scores(const CacheSelect& a, int cus);  // floats of the workspace
+int64_t cache_select_scores(const CacheSelect& a, int cus);      // floats of the workspace
+int64_t cache_select_workgroups(const CacheSelect& a, int cus);  // of its largest launch
 
 hipError_t launch_cache_write(const CacheMove& a, CacheForm form, hipStream_t stream);
 hipError_t launch_cache_read(const CacheMove& a, CacheForm form, hipStream_t stream);

@@ -180,8 +180,8 @@ class Model:
                     for head in range(kv * (heads // h), (kv + 1) * (heads // h)):
                         c = codes[b, head, i]
                         dot = (c.clamp(min=0) * bounds[:, 0] + c.clamp(max=0) * bounds[:, 1]).sum(-1).float() * scales[b, head, i]
-                        score = dot if score is None else torch.maximum(score, dot)
-                    score = torch.where(ok, score * bscale, -math.inf)
+                        score = dot if score is None else torch.fmax(score, dot)
+                    score = torch.where(ok, score * bscale, -math.inf).nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf)
                     best = score.sort(descending=True, stable=True).indices[: budget - 1]
                     chosen = sorted(best.tolist() + [own])
                     out[b, kv, i, : len(chosen)] = torch.tensor(chosen, dtype=torch.int32)

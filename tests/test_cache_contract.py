@@ -299,11 +299,20 @@ def test_c_calls_check_the_cache_pointers(lib) -> None:
                          ("read", ("key", "key_scale", "value", "value_scale")), ("attention", ("key", "key_scale", "value", "value_scale")),
                          ("select", ("bounds", "bound_scale"))):
         for field in fields:
-            for value, message in ((None, "cache pointer is NULL"), (4100, "16-byte aligned")):
+            bad, aligned = (4098, "4-byte aligned") if field == "bound_scale" else (4100, "16-byte aligned")
+            for value, message in ((None, "cache pointer is NULL"), (bad, aligned)):
                 args = _good(name)
                 setattr(args.cache, field, value)
                 with pytest.raises(RuntimeError, match=message):
                     lib.cache_call(name, args, 0)
+
+
+@pytest.mark.parametrize("name", ["write", "read"])
+def test_c_calls_refuse_more_workgroups_than_a_launch_has(lib, name) -> None:
+    args = _good(name)
+    args.cache.kv_heads, args.rows.batch, args.rows.tokens = 1, 1 << 22, 2  # two pages each
+    with pytest.raises(RuntimeError, match="too large for this build"):
+        lib.cache_call(name, args, 0)
 
 
 # ---- index arithmetic --------------------------------------------------------------------------------------------------

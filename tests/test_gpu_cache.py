@@ -12,6 +12,7 @@ import torch
 from _cache import PAGE, Model, table_of, tokens_of, tree_mask
 from _parity import log
 from piper_kernels import QuantizedCache, cache_attention, cache_read, cache_select, cache_write, piper_attention
+from piper_kernels._hip import library as native
 
 pytestmark = pytest.mark.gpu
 
@@ -277,6 +278,90 @@ def test_select_among_many(width, budget, heads, gfx950_device) -> None:
     where = (table, ints(width * PAGE - 3, (width - 9) * PAGE - 2), None)
     got = cache_select(q.to(gfx950_device), cache_of(model, gfx950_device), *on(gfx950_device, *where), budget=budget)
     same(got, model.select(q, *where, budget), "selected")
+
+
+@pytest.mark.parametrize("width, tokens", [(40, 3), (600, 1), (17000, 1)])
+def test_select_with_what_is_not_finite(width, tokens, gfx950_device) -> None:
+    """Heads that are not finite do not count; where none is left, and where a page's scale is any NaN, scores are -inf."""
+    log(f"[case] cache select, not finite, {width}")
+    model = Model(30, 2, 64, INT8)
+    g = torch.Generator().manual_seed(width)
+    model.bounds.copy_(torch.randint(-127, 128, model.bounds.shape, generator=g))
+    model.bound_scale.copy_(torch.rand(model.bound_scale.shape, generator=g))
+    for page, bits in ((3, -1), (8, 0x7FC00000), (11, 0x7F800001), (20, -0x400000)):
+        model.bound_scale[page, 0] = torch.tensor(bits, dtype=torch.int32).view(torch.float32)
+    table = torch.randint(0, 30, (1, width), generator=g, dtype=torch.int32)
+    where = (table, ints(width * PAGE - tokens), None)
+    q = tokens_of(1, 6, tokens, 64, FP16, 66)
+    q[0, 1, 0, 5] = math.inf  # one head of the first K/V head
+    q[0, 3:6, 0, 2] = math.nan  # every head of the second
+    dev = on(gfx950_device, *where)
+    for budget in (2, width // 2, width - 1):
+        got = cache_select(q.to(gfx950_device), cache_of(model, gfx950_device), *dev, budget=budget)
+        same(got, model.select(q, *where, budget), "selected")
+
+
+@pytest.mark.parametrize("codes", [INT8, FP8], ids=["int8", "fp8"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_read_rounds_the_product(d, codes, gfx950_device) -> None:
+    """FP16 reads: code * scale rounded to FP32 and then to FP16, where one rounding of the two gives another value.
+    Scales are made such that for code 3 the exact product is just beside a tie of FP16 and its FP32 value is the tie."""
+    log(f"[case] cache read, ties, D{d} {codes}")
+    tie = torch.arange(1024, 2048, dtype=torch.float64) + 0.5  # between two halves, in [1024, 2048)
+    scale = (tie / 3).float()
+    exact, single = scale.double() * 3, scale * 3
+    apart = (exact != tie) & (single.double() == tie)
+    scale = scale[apart][: 4 * PAGE]
+    assert len(scale) == 4 * PAGE
+    once = torch.from_numpy((scale.double() * 3).numpy().astype("float16"))
+    assert int((once != (scale * 3).half()).sum()) > 50
+    cache = QuantizedCache.allocate(4, 1, d, dtype=codes, device=gfx950_device)
+    three = torch.tensor(3.0).to(codes).view(torch.int8).item()
+    cache.key.view(torch.int8).fill_(three)
+    cache.value.view(torch.int8).fill_(three)
+    cache.key_scale.copy_(scale.view(4, 1, PAGE))
+    cache.value_scale.copy_(scale.view(4, 1, PAGE))
+    table = torch.arange(4, dtype=torch.int32, device=gfx950_device)[None]
+    want = (scale * 3).half()[None, None, :, None].expand(1, 1, 4 * PAGE, d)
+    for x, name in zip(cache_read(cache, table, torch.zeros(1, dtype=torch.int32, device=gfx950_device), size=4 * PAGE, dtype=FP16), ("key", "value")):
+        same(x, want, name)
+
+
+def test_layers_of_one_allocation(gfx950_device) -> None:
+    """The layers of a model as slices of one cache, odd numbers of pages and heads among them."""
+    log("[case] cache layers")
+    layers, pages, d = 3, 3, 64
+    whole = QuantizedCache.allocate(layers * pages, 1, d, device=gfx950_device)
+    table, starts = torch.tensor([[2, 0]], dtype=torch.int32), ints(0)
+    dev = on(gfx950_device, table, starts)
+    for layer in range(layers):
+        cache = QuantizedCache(*(a[layer * pages : (layer + 1) * pages] for a in whole))
+        model = Model(pages, 1, d, INT8)
+        key, value = (tokens_of(1, 1, 100, d, BF16, 70 + 2 * layer + i) for i in (0, 1))
+        cache_write(cache, key.to(gfx950_device), value.to(gfx950_device), *dev)
+        model.write(key, value, table, starts)
+        same_cache(cache, model)
+        q = tokens_of(1, 2, 100, d, BF16, 90 + layer)
+        same(cache_select(q.to(gfx950_device), cache, *dev, budget=1), model.select(q, table, starts, None, 1), "selected")
+
+
+def test_sizes_that_no_launch_has(gfx950_device) -> None:
+    """The workspace functions read no pointer and launch nothing."""
+    lib = native.load_library()
+    cache = native.PiperCache(pages=64, kv_heads=1, head_dim=64, code=native.CACHE_INT8)
+    args_of = {"attention": native.PiperCacheAttentionArgs, "select": native.PiperCacheSelectArgs}
+
+    def bytes_of(name: str, heads: int, batch: int, tokens: int, width: int, **more) -> int:
+        rows = native.PiperCacheRows(table_stride=width, table_width=width, batch=batch, tokens=tokens)
+        args = args_of[name](abi_version=native.CACHE_ABI_VERSION, dtype=native.FLOAT16, heads=heads, cache=cache, rows=rows, **more)
+        return lib.cache_workspace_bytes(name, args)
+
+    assert bytes_of("attention", 8, 2, 4096, 1024) > 0  # shares of a line of blocks' pages
+    assert bytes_of("attention", 8, 2, 4096, 1 << 24) == 0  # whose length 32 bits do not hold: a workgroup a block
+    for name, sizes, more in (("attention", (1, 1 << 23, 1, 4), {}), ("attention", (1, 1 << 10, 1 << 13, 4), {"selected": 4096, "budget": 2}),
+                              ("select", (16, 1 << 13, 1 << 10, 64), {"budget": 2}), ("select", (1, 1 << 13, 4, 1 << 16), {"budget": 2})):
+        with pytest.raises(RuntimeError, match="too large for this build"):
+            bytes_of(name, *sizes, **more)
 
 
 def test_a_cache_beyond_32_bits(gfx950_device) -> None:
