@@ -366,6 +366,7 @@ typedef int int4_t __attribute__((ext_vector_type(4)));
 constexpr int kSelectWaves = 8;
 constexpr int kRowScores = 16384;  // scores in LDS: 64 KiB, two workgroups a CU; also what a workgroup's registers hold
 constexpr int kWaveScores = 1024;  // what one wave's registers hold
+constexpr int kShortWaves = 4, kShortPages = 64;  // of a wave alone: four tiles, which it scores at once
 
 // Scores in the order of whole numbers: the larger the score, the larger the number (-0 is 0, NaN -infinity); all of
 // them above 0, which stands for no score.
@@ -633,6 +634,31 @@ __global__ __launch_bounds__(kWave* kSelectWaves) void cache_select_kernel(Cache
   }
 }
 
+// Short tables: a wave for `tokens` rows, alone.
+template <bool kBf16, int kDim>
+__global__ __launch_bounds__(kWave* kShortWaves) void cache_select_short_kernel(CacheSelect a, int tokens, int columns) {
+  extern __shared__ float scores[];  // [kShortWaves, tokens, table_width]
+  const int wave = threadIdx.x / kWave, per_block = tokens * kShortWaves;
+  const int64_t blocks = (a.rows.tokens + per_block - 1) / per_block;
+  const int first = static_cast<int>(blockIdx.x % blocks) * per_block + wave * tokens;
+  const int64_t unit = blockIdx.x / blocks, b = unit / a.cache.kv_heads, h = unit % a.cache.kv_heads;
+  const int mine = a.rows.tokens - first < tokens ? a.rows.tokens - first : tokens;
+  int most = 0;
+  for (int t = 0; t < mine; ++t) {
+    const int own = own_page(a, b, first + t);
+    most = own > most ? own : most;
+  }
+  const int width = a.rows.table_width;
+  float* const held = scores + static_cast<int64_t>(wave) * tokens * width;
+  if (a.budget > 1 && most >= a.budget)  // else every page is taken
+    score_pages<kBf16, kDim>(a, b, h, first, mine, columns, 0, most, 16, [&](int token, int page, float score) { held[token * width + page] = score; });
+  __threadfence_block();
+  int turn = 0;
+  int32_t* const out = a.output + (unit * a.rows.tokens + first) * a.budget;
+  for (int t = 0; t < mine; ++t)
+    pick_pages<false, kShortPages / kWave>(held + t * width, own_page(a, b, first + t), a.budget, out + static_cast<int64_t>(t) * a.budget, nullptr, turn);
+}
+
 // Longer tables, and few rows of long ones: scores in the workspace, by as many workgroups as there are pages for ...
 constexpr int kScoreTiles = 4;  // of 16 pages, a wave
 
@@ -748,22 +774,34 @@ int64_t cache_select_scores(const CacheSelect& a, int cus) {
   return select_tokens(a, cus) > 0 ? 0 : static_cast<int64_t>(a.batch) * a.cache.kv_heads * a.rows.tokens * a.rows.table_width;
 }
 
+// Whether a wave alone takes its rows: where there are pages for one wave and rows for more.  Eight waves a row's pages
+// leave seven without: 56 sequences of 84 rows and up to 9 pages took 51 us, and 16.9 with a wave each; 18 of 64 rows
+// and 2 pages 17.4 and 6.1.  At 70 pages (8 sequences of 14 rows) a wave alone took 19 us, eight waves 12.3.
+static bool select_short(const CacheSelect& a, int tokens) {
+  return tokens > 0 && a.rows.tokens > tokens && a.rows.table_width <= kShortPages;
+}
+
 // Workgroups for a row's scores in the workspace.
 static int score_parts(const CacheSelect& a) { return static_cast<int>(ceil_div(a.rows.table_width, 4 * kScoreTiles * 16)); }
 
-int64_t cache_select_workgroups(const CacheSelect& a, int cus) {
-  const int64_t units = static_cast<int64_t>(a.batch) * a.cache.kv_heads;
-  const int tokens = select_tokens(a, cus);
-  return tokens > 0 ? units * ceil_div(a.rows.tokens, tokens) : units * a.rows.tokens * score_parts(a);
+int64_t cache_select_most_workgroups(const CacheSelect& a) {
+  return static_cast<int64_t>(a.batch) * a.cache.kv_heads * a.rows.tokens * score_parts(a);
 }
 
 hipError_t launch_cache_select(const CacheSelect& a, CacheForm form, int cus, hipStream_t stream) {
   const int tokens = select_tokens(a, cus), columns = select_columns(a);
-  const dim3 blocks(static_cast<uint32_t>(cache_select_workgroups(a, cus)));
+  const int64_t units = static_cast<int64_t>(a.batch) * a.cache.kv_heads;
+  const dim3 blocks(static_cast<uint32_t>(tokens == 0 ? units * a.rows.tokens * score_parts(a)
+                                                      : units * ceil_div(a.rows.tokens, tokens * (select_short(a, tokens) ? kShortWaves : 1))));
   form.fp8 = false;  // the bounds are INT8 in every cache
   return with_cache_form(form, [&](auto bf16, auto, auto dim) {
     constexpr bool kBf16 = decltype(bf16)::value;
     constexpr int kDim = decltype(dim)::value;
+    if (select_short(a, tokens)) {
+      cache_select_short_kernel<kBf16, kDim>
+          <<<blocks, dim3(kWave * kShortWaves), static_cast<size_t>(kShortWaves) * tokens * a.rows.table_width * 4, stream>>>(a, tokens, columns);
+      return hipGetLastError();
+    }
     if (tokens > 0) {
       cache_select_kernel<kBf16, kDim><<<blocks, dim3(kWave * kSelectWaves), static_cast<size_t>(tokens) * a.rows.table_width * 4, stream>>>(
           a, tokens, columns);
@@ -1009,7 +1047,7 @@ extern "C" int piper_cache_select_workspace_bytes(const piper_cache_select_args*
   int cus = 0, xccs = 0;
   if (int st = piper::device_topology(&cus, &xccs)) return st;
   const piper::CacheSelect select = select_of(*a);
-  if (int st = check_launch(piper::cache_select_workgroups(select, cus))) return st;
+  if (int st = check_launch(piper::cache_select_most_workgroups(select))) return st;
   *bytes = 4 * piper::cache_select_scores(select, cus);
   return PIPER_OK;
 }
@@ -1023,7 +1061,7 @@ extern "C" int piper_cache_select(const piper_cache_select_args* a, void* stream
   const piper::CacheSelect select = select_of(*a);
   int cus = 0, xccs = 0;
   if (int st = piper::device_topology(&cus, &xccs)) return st;
-  if (int st = check_launch(piper::cache_select_workgroups(select, cus))) return st;
+  if (int st = check_launch(piper::cache_select_most_workgroups(select))) return st;
   if (int st = check_workspace(a->workspace, a->workspace_bytes, 4 * piper::cache_select_scores(select, cus))) return st;
   return launched(piper::launch_cache_select(select, form_of(a->cache, a->dtype), cus, static_cast<hipStream_t>(stream)), "cache select");
 }

@@ -92,10 +92,22 @@ __device__ __forceinline__ int wave_prefix(int v) {
   return v;
 }
 
+// Entries of a unit's list up to its last page: what follows that (a list shorter than the budget ends in -1) is not
+// walked through.  1584 lists of up to 5 pages in a budget of 102: 244 us with, 22 without; where lists are full, finding
+// that out takes 0.2 us.
+__device__ __forceinline__ int listed_pages(const CacheAttention& a, int64_t unit) {
+  const int32_t* const list = a.selected + unit * a.budget;
+  int n = 0;
+  for (int from = 0; from < a.budget; from += kWave) {
+    const int i = from + static_cast<int>(threadIdx.x % kWave);
+    const uint64_t pages = __ballot(i < a.budget && list[i < a.budget ? i : 0] >= 0);
+    if (pages != 0) n = from + kWave - __builtin_clzll(pages);
+  }
+  return n;
+}
+
 // Pages of each of a sequence's blocks.
-template <bool kSelected>
 __device__ __forceinline__ int pages_of(const CacheAttention& a, int64_t b) {
-  if (kSelected) return a.budget;
   const int count = a.rows.count(b);
   return count > 0 ? static_cast<int>((a.rows.end(b, count - 1) + kPage - 1) / kPage) : 0;
 }
@@ -116,7 +128,7 @@ template <typename F>
 __device__ __forceinline__ void walk_line(const CacheAttention& a, int block_rows, F f) {
   const int lane = threadIdx.x % kWave, group = a.heads / a.cache.kv_heads, heads = a.cache.kv_heads;
   const auto blocks_of = [&](int64_t b) { return (a.rows.count(b) * group + block_rows - 1) / block_rows; };  // of a head
-  const auto length = [&](int64_t b) { return b < a.batch ? pages_of<false>(a, b) * blocks_of(b) : 0; };  // of a head, in the line
+  const auto length = [&](int64_t b) { return b < a.batch ? pages_of(a, b) * blocks_of(b) : 0; };  // of a head, in the line
   const int length0 = length(lane), prefix0 = wave_prefix(length0);
   int64_t total = __builtin_amdgcn_readlane(prefix0, kWave - 1);
   for (int64_t b0 = kWave; b0 < a.batch; b0 += kWave) total += __builtin_amdgcn_readlane(wave_prefix(length(b0 + lane)), kWave - 1);
@@ -140,7 +152,7 @@ __device__ __forceinline__ void walk_line(const CacheAttention& a, int block_row
       }
     }
     if (found == 0) return;  // starts or counts changed under the kernel
-    int n = pages_of<false>(a, b), blocks = blocks_of(b);
+    int n = pages_of(a, b), blocks = blocks_of(b);
     int block = static_cast<int>((at - first) / n);
     int lo = static_cast<int>((at - first) % n);
     int h = block / blocks;
@@ -160,7 +172,7 @@ __device__ __forceinline__ void walk_line(const CacheAttention& a, int block_row
           h = 0;
           do {  // the line is not at its end: a sequence with rows and pages follows
             if (++b >= a.batch) return;
-            n = pages_of<false>(a, b), blocks = blocks_of(b);
+            n = pages_of(a, b), blocks = blocks_of(b);
           } while (n == 0 || blocks == 0);
         }
       }
@@ -169,30 +181,59 @@ __device__ __forceinline__ void walk_line(const CacheAttention& a, int block_row
   }
   // blocks that do not stand in the line: no pieces, the join makes zeros of them
   for (b = blockIdx.x; b < a.batch; b += a.workgroups) {
-    const int blocks = pages_of<false>(a, b) > 0 ? blocks_of(b) : 0;
+    const int blocks = pages_of(a, b) > 0 ? blocks_of(b) : 0;
     for (int i = threadIdx.x; i < heads * a.blocks_of_unit; i += blockDim.x)
       if (i % a.blocks_of_unit >= blocks) a.pieces[b * heads * a.blocks_of_unit + i] = CachePieces{0, 0};
   }
 }
 
-// Which of kKeys keys a row sees, a bit each: the keys stand `spread(i)` after position `first`, the row sees those before
-// `limit` and, of the drafted ones, those with a true byte in its row of the mask.  All bytes are loaded at once, from
-// clamped places: a load for each visible key alone costs its latency each time.
-template <int kKeys, typename Spread>
-__device__ __forceinline__ uint32_t seen_keys(const CacheAttention& a, const uint8_t* mask_row, int start, int limit, int first, Spread spread) {
+// The lowest n of eight bits, n taken as 0 below 0 and as 8 beyond it.
+__device__ __forceinline__ uint32_t low_bits(int n) { return (1u << (n < 0 ? 0 : n > 8 ? 8 : n)) - 1; }
+
+// Which of four bytes are not 0, a bit each.
+__device__ __forceinline__ uint32_t true_bytes(uint32_t x) {
+  const uint32_t high = (((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x) & 0x80808080u;
+  return (high >> 7) * 0x01020408u >> 24 & 15u;  // bits 8 i to 24 + i; no other product of the two reaches bits 24 to 31
+}
+
+// Which of kRuns runs of eight keys a row sees, a bit each: run r's stand from first + 16 r on, the row sees those before
+// `limit` and, of the drafted ones, those with a true byte in its row of the mask.  A run's bytes are one load, from a
+// place so clamped that all eight are the row's.  (With a load for each byte, and the first page's codes loaded after the
+// queries, a call of one masked page in 320 tile blocks took 31.0 us instead of 28.6, one of two or three 17.1 instead of 14.6.)
+template <int kRuns>
+__device__ __forceinline__ uint32_t seen_keys(const CacheAttention& a, const uint8_t* mask_row, int start, int limit, int first) {
   uint32_t seen = 0;
 #pragma unroll
-  for (int i = 0; i < kKeys; ++i) seen |= static_cast<uint32_t>(first + spread(i) < limit) << i;
+  for (int r = 0; r < kRuns; ++r) seen |= low_bits(limit - (first + 16 * r)) << (8 * r);
   if (mask_row == nullptr) return seen;
-  uint8_t byte[kKeys];
+  uint64_t bytes[kRuns];
+  if (a.rows.tokens >= 8) {
 #pragma unroll
-  for (int i = 0; i < kKeys; ++i) {
-    const int j = first + spread(i) - start;
-    byte[i] = mask_row[j < 0 ? 0 : j < a.rows.tokens ? j : a.rows.tokens - 1];
+    for (int r = 0; r < kRuns; ++r) {
+      const int at = first + 16 * r - start, from = at < 0 ? 0 : at < a.rows.tokens - 8 ? at : a.rows.tokens - 8;
+      __builtin_memcpy(&bytes[r], mask_row + from, 8);
+    }
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+      const int at = first + 16 * r - start, from = at < 0 ? 0 : at < a.rows.tokens - 8 ? at : a.rows.tokens - 8;
+      const int up = from - at < 0 ? 0 : from - at > 7 ? 7 : from - at, down = at - from < 0 ? 0 : at - from > 7 ? 7 : at - from;
+      bytes[r] = bytes[r] << (8 * up) >> (8 * down);  // by more than seven bytes: none of the run's is the row's
+    }
+  } else {
+    uint64_t row = 0;
+#pragma unroll
+    for (int i = 0; i < 7; ++i) row |= static_cast<uint64_t>(mask_row[i < a.rows.tokens ? i : a.rows.tokens - 1]) << (8 * i);
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+      const int at = first + 16 * r - start;
+      bytes[r] = row << (8 * (at >= 0 ? 0 : at < -7 ? 7 : -at)) >> (8 * (at <= 0 ? 0 : at > 7 ? 7 : at));
+    }
   }
 #pragma unroll
-  for (int i = 0; i < kKeys; ++i)
-    if (byte[i] == 0 && first + spread(i) >= start) seen &= ~(1u << i);
+  for (int r = 0; r < kRuns; ++r) {
+    const uint32_t drafted = true_bytes(static_cast<uint32_t>(bytes[r])) | true_bytes(static_cast<uint32_t>(bytes[r] >> 32)) << 4;
+    seen &= ~((~drafted & 0xffu & ~low_bits(start - (first + 16 * r))) << (8 * r));
+  }
   return seen;
 }
 
@@ -495,7 +536,7 @@ __device__ __forceinline__ void cache_stream_block(const CacheAttention& a, cons
       s.load_value(record(page), half);
       uint32_t seen[kTiles];
 #pragma unroll
-      for (int r = 0; r < kTiles; ++r) seen[r] = seen_keys<8>(a, mask_row[r], start, limit[r], base + 8 * s.g, [](int i) { return i; });
+      for (int r = 0; r < kTiles; ++r) seen[r] = seen_keys<1>(a, mask_row[r], start, limit[r], base + 8 * s.g);
       float4_t score[kTiles][2];
       s.scores(score);
       s.template accumulate<true>(score, keys, seen);
@@ -777,6 +818,15 @@ __device__ __forceinline__ void cache_tile_block(const CacheAttention& a, const 
   const int64_t b = piece.b, h = piece.block / a.blocks_of_unit;
   const int start = a.rows.starts[b], count = a.rows.count(b);
   Tile<kBf16, kFp8, kDim, kTileWaves> s(a, shared);
+  // Two pages in turn; a place past the last is loaded from a clamped one, and a page that the table does not name from
+  // page 0 and not used.  The first is on its way before anything waits for the rows.
+  const int32_t* const table = a.rows.page_table + b * a.rows.table_stride;
+  const auto entry = [&](int logical) { return table[logical < a.rows.table_width ? logical : a.rows.table_width - 1]; };
+  const auto is_page = [&](int page) { return page >= 0 && page < a.rows.pages; };
+  const auto record = [&](int page) { return (is_page(page) ? page : 0) * static_cast<int64_t>(a.cache.kv_heads) + h; };
+  int step = piece.lo;
+  int page = entry(step), page1 = entry(step + 1), page2 = entry(step + 2);
+  s.load(record(page));
   const int row = first_row + 32 * (threadIdx.x / kWave) + s.n;
   const int token = row / group;
   const bool real = row < unit_rows && token < count;
@@ -798,16 +848,7 @@ __device__ __forceinline__ void cache_tile_block(const CacheAttention& a, const 
   const int hi = piece.hi < end_page ? piece.hi : end_page;
   const bool busy = __ballot(real) != 0;  // a wave without rows keeps the others' pace
 
-  // Two pages in turn; a place past the last is loaded from a clamped one, and a page that the table does not name from
-  // page 0 and not used.
-  const int32_t* const table = a.rows.page_table + b * a.rows.table_stride;
-  const auto entry = [&](int logical) { return table[logical < a.rows.table_width ? logical : a.rows.table_width - 1]; };
-  const auto is_page = [&](int page) { return page >= 0 && page < a.rows.pages; };
-  const auto record = [&](int page) { return (is_page(page) ? page : 0) * static_cast<int64_t>(a.cache.kv_heads) + h; };
   if (piece.lo < hi) {
-    int step = piece.lo;
-    int page = entry(step), page1 = entry(step + 1), page2 = entry(step + 2);
-    s.load(record(page));
     s.widen(step & 1, most - step * kPage);
     s.load(record(page1));
     __syncthreads();
@@ -829,7 +870,7 @@ __device__ __forceinline__ void cache_tile_block(const CacheAttention& a, const 
     const int limit = real ? static_cast<int>(a.rows.end(b, a.mask != nullptr ? count - 1 : token)) : 0;
     for (; step < hi; ++step) {  // some row sees a part
       if (is_page(page) && busy) {
-        const uint32_t seen = seen_keys<32>(a, mask_row, start, limit, step * kPage, [&](int i) { return 16 * (i / 8) + 8 * s.g + i % 8; });
+        const uint32_t seen = seen_keys<4>(a, mask_row, start, limit, step * kPage + 8 * s.g);
         __builtin_amdgcn_sched_barrier(0);  // its 32 bytes are one register before the scores are more
         s.template use<true>(step & 1, s.reference, seen);
       }
@@ -883,7 +924,7 @@ __device__ __forceinline__ void share_out(const CacheAttention& a, int block_row
   const int64_t unit = blockIdx.x / a.parts;
   const int part = static_cast<int>(blockIdx.x % a.parts);
   const int64_t b = unit / blocks;
-  const int n = pages_of<kList>(a, b);
+  const int n = kList ? listed_pages(a, unit) : pages_of(a, b);
   int parts = (n + a.least_share - 1) / a.least_share;
   parts = parts < 1 ? 1 : parts < a.parts ? parts : a.parts;
   if (part == 0 && threadIdx.x == 0 && a.shares != CacheShares::kWhole) a.pieces[unit] = CachePieces{unit * a.parts, parts};
@@ -970,11 +1011,30 @@ static int64_t unit_rows(const CacheAttention& a) {
 }
 
 // Rows of a block: the stream kernel's 16 or 32 (up to two blocks of them: the second reads its codes from the caches),
-// or the tile kernel's 128 or 256.
+// or the tile kernel's 128 or 256.  Measured at 8 K/V heads of 128 (us):
+//   rows  sequences  context   32 a block  128 a block
+//     48          8     8192         54.5         70.5
+//     64          8     8192         57           72
+//     64          1    16384         24.4         41.5
+//     64         64     4096        180          177
+//     96          8     8192         72 - 75.6    74.6    (three blocks of 32)
+// and with 256 rows, which 128-row blocks read twice: full sequences, 64 of 4096, 454 for 128 and 398 for 256; ragged ones 276
+// and 320; 8 of 8192 143 and 130; one of 16384 65 and 59.
 static int block_rows(const CacheAttention& a) {
   const int64_t rows = unit_rows(a);
   return rows <= 16 ? 16 : rows <= 64 || a.selected != nullptr ? 32 : rows <= 128 ? 128 : 256;
 }
+
+// Up to kUnsplit pages stay one workgroup's: split, they cost the join's launch (4 us; 5 pages in one workgroup 6.6 us, in
+// two and joined 9.4).  Beyond that parts go down to kLeastShare pages, one for each wave: at least 16 a part took 24
+// instead of 14.5 us for 14 blocks of 17 pages, 29 instead of 19.4 for 26 of up to 29.
+//
+// One sequence's blocks, and lists of selected pages, are of a length: equal parts, as many workgroups as a CU takes
+// one of (two of 128 rows).  Two and three a CU took 54.1 and 57.8 instead of 51.8 us for a step of 131072 positions, 35.2 and 37.0
+// instead of 34.8 for selected pages: there are more parts to join.  Sequences of different lengths share a line: one, two and three
+// workgroups a CU took 153, 134 - 139 and 134 - 156 us for 64 steps of up to 8192 positions.  Where there are eight
+// blocks to a place and more, the places fill without splitting.
+constexpr int kUnsplit = 16, kLeastShare = 4;
 
 CacheParts cache_attention_parts(const CacheAttention& a, int head_dim, int cus) {
   const int rows = block_rows(a);
@@ -982,11 +1042,11 @@ CacheParts cache_attention_parts(const CacheAttention& a, int head_dim, int cus)
   CacheParts p{};
   p.blocks_of_unit = ceil_div(unit_rows(a), rows);
   const int64_t blocks = units * p.blocks_of_unit, pages = a.selected != nullptr ? a.budget : a.rows.table_width;
-  p.least_share = 16;
+  p.least_share = kLeastShare;
   p.shares = CacheShares::kWhole;
   p.parts = 1;
   p.workgroups = blocks;
-  if (pages <= p.least_share) return p;
+  if (pages <= kUnsplit) return p;
   if (a.batch == 1 || a.selected != nullptr) {
     const int64_t slots = static_cast<int64_t>(cus) * (rows == 128 ? 2 : 1);
     p.parts = std::min(slots / blocks, ceil_div(pages, p.least_share));
@@ -1030,7 +1090,7 @@ hipError_t launch_cache_attention(const CacheAttention& a, CacheForm form, hipSt
           cache_tile_kernel<kBf16, kFp8, kDim, 8, kPages><<<blocks, dim3(512), 0, stream>>>(a);
       }
       if (const hipError_t err = hipGetLastError(); err != hipSuccess || a.shares == CacheShares::kWhole) return err;
-      if (a.parts > 4)
+      if (a.parts > 4)  // a workgroup a row: else a wave goes through all the parts of one
         cache_join_kernel<kBf16, kDim, kList, kWaves><<<dim3(static_cast<uint32_t>(rows)), threads, 0, stream>>>(a, of_block);
       else
         cache_join_kernel<kBf16, kDim, kList, 1><<<dim3(static_cast<uint32_t>(ceil_div(rows, kWaves))), threads, 0, stream>>>(a, of_block);

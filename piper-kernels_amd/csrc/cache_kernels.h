@@ -72,8 +72,8 @@ struct CacheForm {
   int head_dim;
 };
 
-int64_t cache_select_scores(const CacheSelect& a, int cus);      // floats of the workspace
-int64_t cache_select_workgroups(const CacheSelect& a, int cus);  // of its largest launch
+int64_t cache_select_scores(const CacheSelect& a, int cus);   // floats of the workspace
+int64_t cache_select_most_workgroups(const CacheSelect& a);  // a launch takes no more, whichever kernel it is of
 
 hipError_t launch_cache_write(const CacheMove& a, CacheForm form, hipStream_t stream);
 hipError_t launch_cache_read(const CacheMove& a, CacheForm form, hipStream_t stream);

@@ -223,6 +223,40 @@ def test_attention_to_selected_pages(case, gfx950_device) -> None:
         near(got, *model.attention(q, *where, selected=selected))
 
 
+@pytest.mark.parametrize("rows", [1, 2, 6, 7, 8, 9, 15, 37])
+@pytest.mark.parametrize("heads", [2, 40])
+def test_masks_at_every_place_of_a_page(heads, rows, gfx950_device) -> None:
+    """Drafted tokens from any slot on, across a page's end, fewer and more than a load of the mask has; any byte but 0
+    is true."""
+    log(f"[case] cache attention, masks of {rows} rows, {heads} heads")
+    starts = (0, 1, 5, 8, 29, 56, 60, 63, 64, 123)
+    model, *where = _filled((starts, None, rows, heads, 1, 64, FP16, INT8, "bhtd"), 24)
+    q = tokens_of(len(starts), heads, rows, 64, FP16, 25)
+    mask = torch.rand((len(starts), rows, rows), generator=torch.Generator().manual_seed(26)) < 0.5
+    some = torch.tensor([1, 2, 128, 255], dtype=torch.uint8).repeat(rows * rows)[: rows * rows].view(rows, rows)
+    held = (mask.to(torch.uint8) * some).to(gfx950_device).view(torch.bool)
+    got = cache_attention(q.to(gfx950_device), cache_of(model, gfx950_device), *on(gfx950_device, *where), mask=held)
+    near(got, *model.attention(q, *where, mask=mask))
+
+
+@pytest.mark.parametrize("batch, rows", [(1, 1), (2, 3), (40, 20)])
+def test_lists_shorter_than_their_budget(batch, rows, gfx950_device) -> None:
+    """What follows a list's last page is not walked through: lists of every length, in parts and in one."""
+    log(f"[case] cache attention, short lists, {batch} x {rows}")
+    starts = tuple(600 + 5 * b for b in range(batch))
+    model, *where = _filled((starts, None, rows, 6, 2, 64, BF16, INT8, "bhtd"), 43)
+    q = tokens_of(batch, 6, rows, 64, BF16, 44)
+    cache, dev = cache_of(model, gfx950_device), on(gfx950_device, *where)
+    for budget in (3, 64, 65, 130):
+        g = torch.Generator().manual_seed(budget)
+        selected = torch.randint(0, where[0].shape[1], (batch, 2, rows, budget), generator=g, dtype=torch.int32)
+        length = torch.randint(0, budget + 1, (batch, 2, rows, 1), generator=g)
+        length[0, 0, 0], length[-1, 1, -1] = 0, budget
+        selected = torch.where(torch.arange(budget) < length, selected, -1)
+        got = cache_attention(q.to(gfx950_device), cache, *dev, selected=selected.to(gfx950_device))
+        near(got, *model.attention(q, *where, selected=selected))
+
+
 @pytest.mark.parametrize("codes", [INT8, FP8], ids=["int8", "fp8"])
 def test_attention_beside_bad_pages_and_what_is_not_finite(codes, gfx950_device) -> None:
     """Table entries outside the cache are not seen; a NaN token makes NaN of the rows that see it and no others."""
@@ -278,6 +312,24 @@ def test_select_among_many(width, budget, heads, gfx950_device) -> None:
     where = (table, ints(width * PAGE - 3, (width - 9) * PAGE - 2), None)
     got = cache_select(q.to(gfx950_device), cache_of(model, gfx950_device), *on(gfx950_device, *where), budget=budget)
     same(got, model.select(q, *where, budget), "selected")
+
+
+@pytest.mark.parametrize("width", [1, 16, 63, 64, 65])
+@pytest.mark.parametrize("heads", [1, 3, 8, 20])
+def test_select_of_many_rows_among_few(width, heads, gfx950_device) -> None:
+    """Short tables, a chunk's rows: also rows that the table does not reach, and a count that ends among a wave's."""
+    log(f"[case] cache select of many rows among {width}, {heads}")
+    model = Model(70, 1, 64, INT8)
+    g = torch.Generator().manual_seed(width)
+    model.bounds.copy_(torch.randint(-127, 128, model.bounds.shape, generator=g))
+    model.bound_scale.copy_(torch.rand(model.bound_scale.shape, generator=g))
+    table = torch.randint(0, 70, (3, width), generator=g, dtype=torch.int32)
+    where = (table, ints(width * PAGE - 45, -3, max(0, width * PAGE - 90)), ints(81, 50, 41))
+    q = tokens_of(3, heads, 81, 64, BF16, 64)
+    dev = on(gfx950_device, *where)
+    for budget in (1, 2, width // 2 + 1, width + 3):
+        got = cache_select(q.to(gfx950_device), cache_of(model, gfx950_device), *dev, budget=budget)
+        same(got, model.select(q, *where, budget), "selected")
 
 
 @pytest.mark.parametrize("width, tokens", [(40, 3), (600, 1), (17000, 1)])
