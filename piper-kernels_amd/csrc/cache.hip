@@ -15,6 +15,10 @@ namespace {
 // Both are bound by the bytes they move.  A workgroup has a page of one K/V head, each wave groups of eight of its tokens:
 // lane 8 r + c has an eighth of token r's features, in 32 (D = 128) or 16 consecutive bytes of 16-bit values.  Key
 // codes lie as the lanes have them; value codes change lanes, so that each has all eight tokens of two features or one.
+// Four sequences' 8192 tokens of 8 heads of 128: the write 52 us for 201 MB, 3.9 TB/s, the read 33.  (A token a lane with
+// value codes stored byte by byte: 198 us for the two.)  A pass of the two, 94 us, took 102 with eight waves a workgroup of
+// the write, 98 with the next tokens' loads ahead, 101 with those and two waves, 107 with 64 registers for eight waves a SIMD (13
+// spilled).  One token for each of 64 sequences: 8.4 us, a chain of loads.
 
 constexpr int kMoveWaves = 4;
 
@@ -359,7 +363,9 @@ __global__ __launch_bounds__(kWave* kMoveWaves) void cache_read_kernel(CacheMove
 // head's query heads, token by token; the maximum over a token's columns is one over lanes.  The scores go to LDS and a
 // wave (or for one token all waves) picks the token's pages from registers: the last one's score is found bit by bit,
 // counting with ballots, and the pages come out in their order.  Reading the bounds is what a single token's call has to
-// do; in a chunk the picking, about 20 counts of n / 64 ballots a row, costs as much.
+// do; in a chunk the picking, about 20 counts of n / 64 ballots a row, costs as much.  64 of up to 1024 pages for 128 rows: 11.8 us
+// for the scores (21 MB), 13 for the pages; three bits of a score for each barrier (28 us before, one bit each).  32 of
+// 264 pages for 2000 rows: 20 us.
 
 typedef int int4_t __attribute__((ext_vector_type(4)));
 
@@ -761,7 +767,8 @@ static int select_columns(const CacheSelect& a) {
 
 // Rows of a workgroup whose scores fit its LDS; 0: scores go to the workspace.  That is also the quicker way where there
 // are no more rows than CUs and each has over kSplitPages pages: one workgroup reads a row's bounds at what one CU
-// gets of the memory's rate.
+// gets of the memory's rate.  128 rows of 768 pages took 30.1 us in one kernel, 26.5 in two; of 512 23.8 and 24.1, of 256
+// 21.7 and 22.3.
 constexpr int kSplitPages = 512;
 
 static int select_tokens(const CacheSelect& a, int cus) {

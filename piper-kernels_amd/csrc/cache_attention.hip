@@ -243,6 +243,8 @@ __device__ __forceinline__ uint32_t seen_keys(const CacheAttention& a, const uin
 //   K: lane (m, g) = (lane % 16, lane / 16) takes 16 bytes of row key(m), features 64 c + 16 g on.  Row m of tile t is
 //      key 8 (m / 4) + 4 t + m % 4 of the half page: then column n's lane (n, g) holds keys 8 g + 0..7.
 //   V: lane (m, g) takes 16 bytes: keys 8 g + 0..7 of features 32 f + 2 m and 32 f + 2 m + 1.
+// Bound by the codes' reading: one step at 131072 positions (8 K/V heads of 128) 45.6 us, 6.1 TB/s; 64 steps of up to 8191
+// 131.7, 5.3 TB/s.  Plain instead of nontemporal loads read pages at 6.1 instead of 6.8 TB/s.
 template <bool kBf16, bool kFp8, int kDim, int kTiles>
 struct Stream {
   static constexpr int kChunks = kDim / 64, kFeatures = kDim / 32;  // K pieces of a row; pairs of V tiles
@@ -603,6 +605,9 @@ __device__ __forceinline__ void cache_stream_block(const CacheAttention& a, cons
 // codes, loaded a page earlier, are widened into the other, and the ones after that are loaded.  S^T = K Q^T and
 // O^T = V^T P^T on 32x32x16 instructions; lane (n, g) = (lane % 32, lane / 32) holds of row n the keys 16 p + 8 g + 0..7
 // of each 32.
+// Bound by VALU issue (widening, softmax, P: 55 - 69% of the time) beside the matrix instructions (33 - 36%), which hide only part of
+// it: 2048 rows of 32 heads on 8 of 128 after 32768 positions 1266 us, 896 TFLOP/s, 1.33 ms with each read just before its
+// matrix instruction.  Waves in opposite halves of a page took 1.31 - 1.50 ms, 16 rows a wave at four waves a SIMD 1.76.
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
