@@ -616,8 +616,9 @@ __global__ __launch_bounds__(kWave* kSelectWaves) void cache_select_kernel(Cache
   }
   const int width = a.rows.table_width;
   if (a.budget > 1 && most >= a.budget)  // else every page is taken
-    score_pages<kBf16, kDim>(a, b, h, first, mine, columns, 16 * wave, most, 16 * kSelectWaves,
-                             [&](int token, int page, float score) { scores[token * width + page] = score; });
+    for (int from = 0, per = 16 / columns; from < mine; from += per)
+      score_pages<kBf16, kDim>(a, b, h, first + from, mine - from < per ? mine - from : per, columns, 16 * wave, most, 16 * kSelectWaves,
+                               [&](int token, int page, float score) { scores[(from + token) * width + page] = score; });
   __syncthreads();
   int turn = 0;
   int32_t* const out = a.output + (unit * a.rows.tokens + first) * a.budget;
@@ -774,7 +775,13 @@ constexpr int kSplitPages = 512;
 static int select_tokens(const CacheSelect& a, int cus) {
   const int64_t rows = static_cast<int64_t>(a.batch) * a.cache.kv_heads * a.rows.tokens;
   if (a.rows.table_width > kRowScores || (rows <= cus && a.rows.table_width > kSplitPages)) return 0;
-  return std::min(std::min(16 / select_columns(a), kRowScores / a.rows.table_width), a.rows.tokens);
+  int tokens = std::min(std::min(16 / select_columns(a), kRowScores / a.rows.table_width), a.rows.tokens);
+  // A tile's rows; or more, so that each wave picks a row's pages, where a wave holds a row's scores and two workgroups a
+  // CU remain.  5664 rows of 16 heads and 258 pages, a row a workgroup, took 290 us, eight a workgroup 207.
+  while (a.rows.table_width > kShortPages && a.rows.table_width <= kWaveScores && 2 * tokens <= kSelectWaves &&
+         2 * tokens * a.rows.table_width <= kRowScores && rows / (2 * tokens) >= 2 * static_cast<int64_t>(cus))
+    tokens *= 2;
+  return tokens;
 }
 
 int64_t cache_select_scores(const CacheSelect& a, int cus) {

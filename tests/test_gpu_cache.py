@@ -332,6 +332,21 @@ def test_select_of_many_rows_among_few(width, heads, gfx950_device) -> None:
         same(got, model.select(q, *where, budget), "selected")
 
 
+@pytest.mark.parametrize("width, heads, rows", [(66, 16, 2101), (66, 3, 4500), (65, 32, 1100), (64, 16, 2101), (1024, 16, 1050)])
+def test_select_of_a_long_chunk(width, heads, rows, gfx950_device) -> None:
+    """More rows than workgroups: several tiles' rows in each, and the last of them ends early."""
+    log(f"[case] cache select of {rows} rows among {width}, {heads} heads")
+    model = Model(70, 1, 64, INT8)
+    g = torch.Generator().manual_seed(width + rows)
+    model.bounds.copy_(torch.randint(-127, 128, model.bounds.shape, generator=g))
+    model.bound_scale.copy_(torch.rand(model.bound_scale.shape, generator=g))
+    table = torch.randint(0, 70, (1, width), generator=g, dtype=torch.int32)
+    where = (table, ints(width * PAGE - rows + 7), ints(rows - 3))
+    q = tokens_of(1, heads, rows, 64, BF16, 65)
+    got = cache_select(q.to(gfx950_device), cache_of(model, gfx950_device), *on(gfx950_device, *where), budget=9)
+    same(got, model.select(q, *where, 9), "selected")
+
+
 @pytest.mark.parametrize("width, tokens", [(40, 3), (600, 1), (17000, 1)])
 def test_select_with_what_is_not_finite(width, tokens, gfx950_device) -> None:
     """Heads that are not finite do not count; where none is left, and where a page's scale is any NaN, scores are -inf."""
